@@ -32,6 +32,17 @@ torch::Tensor paged_attention_decode_strided(
     torch::Tensor kcache, torch::Tensor vcache, torch::Tensor block_tables,
     torch::Tensor ctx_lens, double scale);
 bool kv_copy_page(torch::Tensor key, torch::Tensor value, int64_t src, std::vector<int64_t> dst);
+torch::Tensor paged_attention_chunk(torch::Tensor q, torch::Tensor kcache,
+                                    torch::Tensor vcache,
+                                    torch::Tensor block_tables,
+                                    torch::Tensor cu, torch::Tensor ctx_lens,
+                                    double scale, int64_t longest);
+std::vector<torch::Tensor> chunk_slots(torch::Tensor block_tables,
+                                       torch::Tensor ctx_lens,
+                                       torch::Tensor new_lens,
+                                       torch::Tensor pages, int64_t block_size,
+                                       int64_t rows,
+                                       c10::optional<torch::Tensor> held);
 void kv_cache_scatter(torch::Tensor k, torch::Tensor v,
                       torch::Tensor key_cache, torch::Tensor value_cache,
                       torch::Tensor slot_mapping);
@@ -210,6 +221,13 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("kv_cache_scatter", &kv_cache_scatter, "paged KV cache scatter");
   m.def("paged_attention_decode", &paged_attention_decode,
         "paged GQA decode attention");
+  m.def("paged_attention_chunk", &paged_attention_chunk,
+        "causal GQA attention of chunks of new tokens over the paged cache");
+  m.def("chunk_slots", &chunk_slots,
+        "block tables, positions and cache rows of a step's new tokens",
+        py::arg("block_tables"), py::arg("context_lens"), py::arg("new_lens"),
+        py::arg("pages"), py::arg("block_size"), py::arg("rows"),
+        py::arg("held") = py::none());
   m.def("sample_tokens", &sample_tokens,
         "fused temperature/top-k/top-p categorical sampling");
   m.def("logprob_lse_fwd", &logprob_lse_fwd,

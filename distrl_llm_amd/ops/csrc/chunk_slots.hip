@@ -1,0 +1,178 @@
+// Where a step's new tokens lie in the paged cache, from the requests' lengths: rows of
+// the flat batch, positions, cache rows, and the block tables' next pages.
+//
+// Request b has ctx[b] tokens in the cache and brings new[b]; its pages are ceil(n / block)
+// entries of its table, of which held[b] are there. What it is short of comes from a list
+// of free pages, one request's behind the other's:
+//   cu[b] = sum of new[< b],  opened[b] = sum of (ceil((ctx + new) / block) - held)[< b].
+// Every workgroup forms both sums for itself in LDS (lengths of 1000 requests are 12 KB, in
+// every L2 after the first), so that one launch is all; then a thread takes a token, or a
+// page that is opened, and looks for its request there.
+#include <torch/extension.h>
+#include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGuard.h>
+#include "common.h"
+
+namespace {
+
+constexpr int THREADS = 256, MOST = 8192;       // requests: two sums of 32 KB in LDS
+
+struct Slots {
+  int* tables;                  // (B, width)
+  const int *ctx, *fresh, *held, *pages;        // held: or null, what ctx fills
+  int *positions, *cu, *context;
+  int64_t *slots, *last;
+  int B, width, block, free, rows;
+};
+
+struct Need { int tokens, pages; };
+
+DEV_INLINE int pages_of(int n, int block) { return n <= 0 ? 0 : (n - 1) / block + 1; }
+DEV_INLINE int held_of(const Slots& a, int b) {
+  return max(0, a.held ? a.held[b] : pages_of(a.ctx[b], a.block));
+}
+DEV_INLINE Need need_of(const Slots& a, int b) {
+  const int n = max(0, a.fresh[b]);
+  return {n, max(0, pages_of(a.ctx[b] + n, a.block) - held_of(a, b))};
+}
+
+// the largest b < n with sum[b] <= i; sums never fall, sum[0] = 0
+DEV_INLINE int find(const int* sum, int n, int i) {
+  int lo = 0;
+  while (n > 1) {
+    const int h = n / 2;
+    if (sum[lo + h] <= i) {
+      lo += h;
+      n -= h;
+    } else {
+      n = h;
+    }
+  }
+  return lo;
+}
+
+__global__ __launch_bounds__(THREADS)
+void chunk_slots_kernel(Slots a) {
+  extern __shared__ int lds[];
+  int *cu = lds, *opened = lds + a.B + 1;
+  __shared__ Need wave_sum_of[THREADS / WAVE];
+  const int tid = threadIdx.x, lane = tid & (WAVE - 1), wave = tid / WAVE;
+  // a run of requests a thread, then the runs' sums over the workgroup
+  const int run = CDIV(a.B, THREADS), b0 = min(tid * run, a.B), b1 = min(b0 + run, a.B);
+  Need sum{0, 0};
+  for (int b = b0; b < b1; ++b) {
+    const Need n = need_of(a, b);
+    sum.tokens += n.tokens;
+    sum.pages += n.pages;
+  }
+  Need to = sum;                // inclusive over the wave
+  #pragma unroll
+  for (int off = 1; off < WAVE; off <<= 1) {
+    const int t = __shfl_up(to.tokens, off, WAVE), p = __shfl_up(to.pages, off, WAVE);
+    if (lane >= off) {
+      to.tokens += t;
+      to.pages += p;
+    }
+  }
+  if (lane == WAVE - 1) wave_sum_of[wave] = to;
+  __syncthreads();
+  Need at{to.tokens - sum.tokens, to.pages - sum.pages};
+  for (int w = 0; w < wave; ++w) {
+    at.tokens += wave_sum_of[w].tokens;
+    at.pages += wave_sum_of[w].pages;
+  }
+  for (int b = b0; b < b1; ++b) {
+    cu[b] = at.tokens;
+    opened[b] = at.pages;
+    const Need n = need_of(a, b);
+    at.tokens += n.tokens;
+    at.pages += n.pages;
+  }
+  if (tid == THREADS - 1) {
+    cu[a.B] = at.tokens;
+    opened[a.B] = at.pages;
+  }
+  __syncthreads();
+
+  const int total = cu[a.B], stride = gridDim.x * THREADS, me = blockIdx.x * THREADS + tid;
+  for (int i = me; i < a.rows; i += stride) {
+    int position = 0;
+    int64_t slot = -1;
+    if (i < total) {
+      const int b = find(cu, a.B, i);
+      position = a.ctx[b] + i - cu[b];
+      const int p = position / a.block, held = held_of(a, b);
+      const int from = opened[b] + p - held;
+      int page = -1;
+      if (position >= 0 && p < a.width)
+        page = p < held ? a.tables[(int64_t)b * a.width + p]
+                        : (unsigned)from < (unsigned)a.free ? a.pages[from] : -1;
+      if (page >= 0) slot = (int64_t)page * a.block + position % a.block;
+    }
+    a.positions[i] = position;
+    a.slots[i] = slot;
+  }
+  for (int i = me; i < opened[a.B]; i += stride) {
+    const int b = find(opened, a.B, i), p = held_of(a, b) + i - opened[b];
+    if ((unsigned)p < (unsigned)a.width) a.tables[(int64_t)b * a.width + p] = i < a.free ? a.pages[i] : -1;
+  }
+  for (int b = me; b <= a.B; b += stride) {
+    a.cu[b] = min(cu[b], a.rows);
+    if (b == a.B) break;
+    a.context[b] = a.ctx[b] + max(0, a.fresh[b]);
+    a.last[b] = min(max(cu[b + 1], 1), max(a.rows, 1)) - 1;
+  }
+}
+
+}  // namespace
+
+// {positions (rows) int32, slots (rows) int64, cu (B + 1) int32, context lengths after the
+// step (B) int32, each request's last row (B) int64}; block_tables <- the opened pages.
+std::vector<torch::Tensor> chunk_slots(torch::Tensor block_tables, torch::Tensor ctx_lens,
+                                       torch::Tensor new_lens, torch::Tensor pages,
+                                       int64_t block_size, int64_t rows,
+                                       c10::optional<torch::Tensor> held) {
+  TORCH_CHECK(block_tables.is_cuda() && block_tables.dim() == 2,
+              "chunk_slots: block_tables (requests, pages) on the GPU");
+  const int64_t B = block_tables.size(0), width = block_tables.size(1);
+  auto check = [&](const torch::Tensor& t, int64_t n, const char* what) {
+    TORCH_CHECK(t.device() == block_tables.device() && t.scalar_type() == at::kInt &&
+                t.is_contiguous() && t.numel() == n, "chunk_slots: ", what, ": device, type, size or layout");
+  };
+  check(block_tables, B * width, "block_tables");
+  check(ctx_lens, B, "context_lens");
+  check(new_lens, B, "new_lens");
+  check(pages, pages.numel(), "pages");
+  if (held) check(*held, B, "held");
+  TORCH_CHECK(block_size > 0 && block_size < (1ll << 31), "chunk_slots: block_size");
+  TORCH_CHECK(rows >= 0 && rows < (1ll << 31) - (1 << 24) && pages.numel() < (1ll << 31),
+              "chunk_slots: rows");
+  TORCH_CHECK(B <= MOST, "chunk_slots: up to ", MOST, " requests");
+  const c10::cuda::CUDAGuard guard(block_tables.device());
+  auto ints = block_tables.options();
+  auto longs = ints.dtype(at::kLong);
+  auto positions = torch::empty({rows}, ints), cu = torch::empty({B + 1}, ints);
+  auto context = torch::empty({B}, ints);
+  auto slots = torch::empty({rows}, longs), last = torch::empty({B}, longs);
+  Slots a{};
+  a.tables = block_tables.data_ptr<int>();
+  a.ctx = ctx_lens.data_ptr<int>();
+  a.fresh = new_lens.data_ptr<int>();
+  a.held = held ? held->data_ptr<int>() : nullptr;
+  a.pages = pages.data_ptr<int>();
+  a.positions = positions.data_ptr<int>();
+  a.cu = cu.data_ptr<int>();
+  a.context = context.data_ptr<int>();
+  a.slots = slots.data_ptr<int64_t>();
+  a.last = last.data_ptr<int64_t>();
+  a.B = B;
+  a.width = width;
+  a.block = block_size;
+  a.free = pages.numel();
+  a.rows = rows;
+  const int64_t work = std::max(std::max(rows, B + 1), std::min<int64_t>(pages.numel(), B * width));
+  hipLaunchKernelGGL(chunk_slots_kernel, dim3(std::min<int64_t>(CDIV(work, THREADS), 1024)),
+                     dim3(THREADS), 2 * (B + 1) * sizeof(int), at::cuda::getCurrentCUDAStream(), a);
+  HIP_CHECK_LAST();
+  return {positions, slots, cu, context, last};
+}

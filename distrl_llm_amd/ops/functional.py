@@ -9,7 +9,7 @@ Set ``DISTRL_ALLOW_EAGER_GPU=1`` only for debugging.
 from __future__ import annotations
 
 import os
-from typing import Optional, Tuple
+from typing import NamedTuple, Optional, Tuple
 
 import torch
 
@@ -155,6 +155,83 @@ def paged_attention_decode(q, key_cache, value_cache, block_tables,
                 float(scale))
     return R.paged_attention_decode(q, key_cache, value_cache, block_tables,
                                     context_lens, scale)
+
+
+# ------------------------------------------- chunks over a paged cache
+
+def paged_attention_chunk(q, key_cache, value_cache, block_tables, cu,
+                          context_lens, scale: float, longest: int) -> torch.Tensor:
+    """Causal GQA attention of chunks of new tokens over the paged cache
+    (ops/csrc/chunk_attn.hip): the tokens behind a cached prefix, the next
+    chunk of a long prompt, single tokens, in one batch.
+
+    q (T, H, D) in any strides: sequence b's new tokens are rows cu[b] ..
+    cu[b + 1], cu (B + 1,). Their keys and values are in the caches (pages,
+    block, KV, D) already; block_tables (B, width) has each sequence's pages,
+    context_lens (B,) its tokens in the cache with the new ones. The token at
+    position p sees keys 0 .. p, as far as its table reaches; a page number
+    outside the cache reads as zeros, a token that sees no key and rows of no
+    sequence give zeros. Cached values a sequence has have to be finite; what
+    lies behind its end or on other pages may be anything. ``longest``: the
+    most rows of one sequence; it picks the kernel, not the result's rows.
+
+    bfloat16 and head_dim 64 or 128 on the GPU. No gradient: the cache serves
+    generation."""
+    if torch.is_grad_enabled() and any(
+            t.requires_grad for t in (q, key_cache, value_cache)):
+        raise RuntimeError("paged_attention_chunk has no gradient: call it "
+                           "under torch.no_grad()")
+    if not 0.0 < scale < 1e30 or longest < 0:
+        raise ValueError("paged_attention_chunk: a positive scale, longest >= 0")
+    if q.is_cuda:
+        ext = _require_ext("paged_attention_chunk")
+        if ext is not None:
+            return ext.paged_attention_chunk(
+                q, key_cache, value_cache, block_tables.to(torch.int32).contiguous(),
+                cu.to(torch.int32).contiguous(),
+                context_lens.to(torch.int32).contiguous(), float(scale), int(longest))
+    return R.paged_attention_chunk(q, key_cache, value_cache, block_tables, cu,
+                                   context_lens, scale)
+
+
+class ChunkSlots(NamedTuple):
+    positions: torch.Tensor      # (rows,) int32; 0 behind the last request
+    slots: torch.Tensor          # (rows,) int64 cache rows; -1: none
+    cu: torch.Tensor             # (B + 1,) int32, first row of every request
+    context_lens: torch.Tensor   # (B,) int32, with the new tokens
+    last: torch.Tensor           # (B,) int64, each request's last row
+
+
+def chunk_slots(block_tables, context_lens, new_lens, pages, block_size: int,
+                rows: int, held=None) -> ChunkSlots:
+    """Where a step's new tokens lie in the paged cache, from the requests'
+    lengths (ops/csrc/chunk_slots.hip), one launch: request b has
+    context_lens[b] tokens there and brings new_lens[b], its rows of the flat
+    batch one request behind the other.
+
+    block_tables (B, width) is written in place: its rows hold ``held`` pages
+    each (default: those that context_lens fill), and what a request is short
+    of is taken from ``pages``, request by request. All are int32 and
+    contiguous. ``rows``: rows of the batch; those behind the last request,
+    tokens past a table's end and those whose page is missing or negative get
+    cache row -1, which the writers of the cache skip. A request without new
+    tokens has the row before it as its last one."""
+    for t in (block_tables, context_lens, new_lens, pages, held):
+        if t is not None and (t.dtype != torch.int32 or not t.is_contiguous()
+                              or t.device != block_tables.device):
+            raise ValueError("chunk_slots: int32, contiguous, on one device")
+    if block_tables.dim() != 2 or block_size <= 0 or rows < 0 or any(
+            t is not None and t.shape != block_tables.shape[:1]
+            for t in (context_lens, new_lens, held)):
+        raise ValueError("chunk_slots: block_tables (requests, pages), a length "
+                         "for each request, a block size and rows")
+    if block_tables.is_cuda:
+        ext = _require_ext("chunk_slots")
+        if ext is not None:
+            return ChunkSlots(*ext.chunk_slots(block_tables, context_lens, new_lens,
+                                               pages, int(block_size), int(rows), held))
+    return ChunkSlots(*R.chunk_slots(block_tables, context_lens, new_lens, pages,
+                                     block_size, rows, held))
 
 
 # -------------------------------------------------------------- sampling

@@ -113,6 +113,71 @@ def paged_attention_decode(q: torch.Tensor, key_cache: torch.Tensor,
     return out.to(q.dtype)
 
 
+def paged_attention_chunk(q: torch.Tensor, key_cache: torch.Tensor,
+                          value_cache: torch.Tensor, block_tables: torch.Tensor,
+                          cu: torch.Tensor, context_lens: torch.Tensor,
+                          scale: float) -> torch.Tensor:
+    """Causal attention of chunks of new tokens over the paged KV pool, see
+    ``functional.paged_attention_chunk``: sequence by sequence."""
+    rows, n_heads, head_dim = q.shape
+    num_blocks, block_size, n_kv = key_cache.shape[:3]
+    group = n_heads // n_kv
+    reach = block_tables.shape[1] * block_size
+    out = torch.zeros(rows, n_heads, head_dim, dtype=q.dtype, device=q.device)
+    firsts = [min(max(int(c), 0), rows) for c in cu]
+    for s, (first, end) in enumerate(zip(firsts, firsts[1:])):
+        before = int(context_lens[s]) - (end - first)
+        keys = min(before + end - first, reach)
+        if end <= first or keys <= 0:
+            continue
+        at = torch.arange(keys, device=q.device)
+        page = block_tables[s].long()[at // block_size]
+        there = ((page >= 0) & (page < num_blocks)).view(-1, 1, 1)
+        line = page.clamp(0, num_blocks - 1) * block_size + at % block_size
+        k, v = (torch.where(there, c.reshape(-1, n_kv, head_dim)[line].float(), 0.0)
+                .repeat_interleave(group, dim=1).transpose(0, 1)
+                for c in (key_cache, value_cache))              # (H, keys, D)
+        scores = q[first:end].float().transpose(0, 1) @ k.transpose(1, 2) * scale
+        place = before + torch.arange(end - first, device=q.device)
+        scores = scores.masked_fill(at > place[:, None], float("-inf"))
+        o = (scores.softmax(-1) @ v).transpose(0, 1)
+        out[first:end] = torch.where((place >= 0).view(-1, 1, 1), o, 0.0).to(q.dtype)
+    return out
+
+
+def chunk_slots(block_tables: torch.Tensor, context_lens: torch.Tensor,
+                new_lens: torch.Tensor, pages: torch.Tensor, block_size: int,
+                rows: int, held: Optional[torch.Tensor] = None):
+    """Where a step's new tokens lie in the paged cache, see
+    ``functional.chunk_slots``: token by token."""
+    width, dev = block_tables.shape[1], block_tables.device
+    free, at = pages.tolist(), 0
+    positions, slots, cu = [], [], [0]
+    for b, (ctx, new) in enumerate(zip(context_lens.tolist(), new_lens.tolist())):
+        new = max(new, 0)
+        have = -(-ctx // block_size) if held is None else int(held[b])
+        table = block_tables[b].tolist()
+        for p in range(max(have, 0), -(-(ctx + new) // block_size)):
+            page = free[at] if at < len(free) else -1
+            at += 1
+            if p < width:
+                table[p] = page
+        block_tables[b] = torch.tensor(table, dtype=torch.int32, device=dev)
+        for position in range(ctx, ctx + new):
+            p = position // block_size
+            page = table[p] if 0 <= p < width else -1
+            positions.append(position)
+            slots.append(page * block_size + position % block_size if page >= 0 else -1)
+        cu.append(cu[-1] + new)
+    spare = max(rows - len(slots), 0)
+    return (torch.tensor((positions + [0] * spare)[:rows], dtype=torch.int32, device=dev),
+            torch.tensor((slots + [-1] * spare)[:rows], dtype=torch.int64, device=dev),
+            torch.tensor([min(c, rows) for c in cu], dtype=torch.int32, device=dev),
+            (context_lens + new_lens.clamp_min(0)).to(torch.int32),
+            torch.tensor([min(max(c, 1), max(rows, 1)) - 1 for c in cu[1:]],
+                         dtype=torch.int64, device=dev))
+
+
 def varlen_prefill_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
                              seq_lens, scale: float) -> torch.Tensor:
     """Causal attention over concatenated variable-length prompts.

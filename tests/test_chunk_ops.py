@@ -1,0 +1,383 @@
+"""Prompts over a paged cache: attention of chunks of new tokens and the layout of
+their cache rows, against plain forms in 64 bits.
+
+Tolerance of the attention on the GPU (bf16 in and out, fp32 sums): the result's
+rounding is off by up to half a step, 2^-8 relative to it, and a weight's rounding to
+bf16 by 2^-8 of the weight, so the sum of weights times |v| by 2^-8 of that sum; fp32
+sums of up to 2^15 products with the running maximum's rescaling stay below 2^-12 of
+it. So |o - exact| <= 2^-8 |exact| + (2^-8 + 2^-12) sum w |v|, element by element,
+where scores themselves are off by far less than a bf16 step: a score is a sum of
+D <= 128 exact products, off by up to 2^-17 of sum |q k| scale, and at |q|, |k| of
+about one that is below 2^-12. The CPU path computes in fp32 throughout: there a score
+of D = 16 products is off by up to 16 2^-24 sum |q k| scale < 2^-18, its weight by twice
+that with the sum's, and sums of up to 371 weighed values by 371 2^-24 < 2^-15 of
+sum w |v|: 2^-14 in all."""
+
+import math
+
+import pytest
+import torch
+
+from distrl_llm_amd.ops import functional as OF
+
+HEADS = [(8, 2, 64), (14, 2, 64), (12, 2, 128), (28, 4, 128), (8, 8, 64), (64, 8, 128),
+         (5, 1, 128)]
+
+
+def make(heads, kv, dim, block, new, cached, seed=0, device="cpu", dtype=torch.bfloat16,
+         spare=2, stale=float("nan"), pad_rows=0):
+    """Requests with pages in a shuffled order; what no token fills is `stale`."""
+    g = torch.Generator().manual_seed(seed)
+    lens = [n + c for n, c in zip(new, cached)]
+    needed = [-(-n // block) for n in lens]
+    width = max(needed + [1]) + spare
+    pages = torch.randperm(sum(needed) + 3, generator=g).tolist()
+    key = torch.full((len(pages), block, kv, dim), stale)
+    value = key.clone()
+    tables = torch.full((len(new), width), 10 ** 6, dtype=torch.int32)
+    for b, (n, p) in enumerate(zip(lens, needed)):
+        for i in range(p):
+            page = pages.pop()
+            tables[b, i] = page
+            filled = min(block, n - i * block)
+            key[page, :filled] = torch.randn(filled, kv, dim, generator=g)
+            value[page, :filled] = torch.randn(filled, kv, dim, generator=g)
+    rows = sum(new) + pad_rows
+    packed = torch.randn(rows, (heads + 2 * kv) * dim, generator=g).to(device, dtype)
+    cu = torch.tensor([0] + new).cumsum(0).to(torch.int32)
+    return dict(q=packed[:, :heads * dim].unflatten(1, (heads, dim)),
+                key_cache=key.to(device, dtype), value_cache=value.to(device, dtype),
+                block_tables=tables.to(device), cu=cu.to(device),
+                context_lens=torch.tensor(lens, dtype=torch.int32, device=device),
+                scale=dim ** -0.5, longest=max(new + [0]))
+
+
+def exact(q, key_cache, value_cache, block_tables, cu, context_lens, scale, longest):
+    """(result, sum of weights times |v|) in 64 bits on the CPU, row by row of a head's
+    keys: softmax over those that a token sees."""
+    q, tables = q.cpu().double(), block_tables.cpu().tolist()
+    cu, lens = cu.tolist(), context_lens.tolist()
+    pages, block, kv, dim = key_cache.shape
+    heads = q.shape[1]
+    cache = [c.cpu().double().view(-1, kv, dim) for c in (key_cache, value_cache)]
+    out = torch.zeros(2, *q.shape, dtype=torch.float64)
+    for b, (first, end) in enumerate(zip(cu, cu[1:])):
+        before = lens[b] - (end - first)
+        keys = min(lens[b], len(tables[b]) * block)
+        line = [tables[b][j // block] * block + j % block
+                if 0 <= tables[b][j // block] < pages else -1 for j in range(max(keys, 0))]
+        k, v = (torch.stack([c[i] if i >= 0 else torch.zeros(kv, dim, dtype=torch.float64)
+                             for i in line]) if line else c[:0] for c in cache)
+        for t in range(first, end):
+            n = min(before + t - first + 1, keys)
+            if n <= 0:
+                continue
+            qt = q[t].view(kv, heads // kv, dim)
+            w = torch.softmax(torch.matmul(qt, k[:n].permute(1, 2, 0)) * scale, -1)
+            for i, x in enumerate((v[:n], v[:n].abs())):
+                out[i, t] = torch.matmul(w, x.transpose(0, 1)).reshape(heads, dim)
+    return out[0], out[1]
+
+
+def check(case, got):
+    want, size = exact(**case)
+    bound = want.abs() * 2.0 ** -8 + size * (2.0 ** -8 + 2.0 ** -12) + 1e-30
+    if case["q"].dtype == torch.float32:
+        bound = size * 2.0 ** -14 + 1e-30
+    off = (got.cpu().double() - want).abs()
+    assert bool((off <= bound).all()), float((off / bound).max())
+
+
+EDGES = [
+    ([1], [0]), ([1], [1]), ([1], [15]), ([1], [16]), ([2], [63]), ([5], [64]),
+    ([17, 1, 33], [0, 40, 7]), ([0, 3, 0], [5, 0, 0]), ([130], [0]), ([64], [64]),
+    ([1, 1, 1, 70], [300, 5, 64, 129]),
+]
+
+
+@pytest.mark.parametrize("block", [1, 5, 16])
+@pytest.mark.parametrize("new,cached", EDGES)
+def test_attention_cpu(new, cached, block):
+    case = make(4, 2, 16, block, new, cached, seed=len(new) + block, dtype=torch.float32)
+    check(case, OF.paged_attention_chunk(**case))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("block", [1, 16, 24, 128])
+@pytest.mark.parametrize("heads,kv,dim", HEADS)
+@pytest.mark.parametrize("new,cached", EDGES)
+def test_attention(new, cached, heads, kv, dim, block):
+    case = make(heads, kv, dim, block, new, cached, seed=sum(new) + heads, device="cuda")
+    check(case, OF.paged_attention_chunk(**case))
+
+
+LONG = [([1], [5000]), ([1, 1], [8191, 300]), ([3, 200], [4000, 9000]), ([33], [2500]),
+        ([9, 0, 1], [0, 700, 6000])]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("heads,kv,dim", [(14, 2, 64), (28, 4, 128), (64, 8, 128)])
+@pytest.mark.parametrize("new,cached", LONG)
+def test_attention_long(new, cached, heads, kv, dim):
+    """Contexts that are cut into slices and joined."""
+    case = make(heads, kv, dim, 16, new, cached, seed=heads, device="cuda")
+    check(case, OF.paged_attention_chunk(**case))
+
+
+@pytest.mark.gpu
+def test_attention_of_many_sequences():
+    """More than 64 x 64 of them, some without rows, and rows of none behind."""
+    n = 4500
+    new = [(i * 5) % 3 for i in range(n)]
+    case = make(4, 2, 64, 4, new, [(i * 7) % 6 for i in range(n)], device="cuda", pad_rows=300)
+    got = OF.paged_attention_chunk(**case)
+    check(case, got)
+    assert not bool(got[sum(new):].any())
+
+
+@pytest.mark.gpu
+def test_attention_of_strided_queries():
+    case = make(8, 2, 64, 16, [20, 3], [40, 100], device="cuda")
+    want = OF.paged_attention_chunk(**case)
+    q = case["q"]
+    heads_first = q.transpose(0, 1).contiguous().transpose(0, 1)
+    odd = torch.empty(q.shape[0], 8, 65, dtype=q.dtype, device="cuda")[..., 1:]
+    odd.copy_(q)
+    wide = torch.empty(q.shape[0], 8, 128, dtype=q.dtype, device="cuda")[..., ::2]
+    wide.copy_(q)
+    for other in (heads_first, odd, wide, q.contiguous()):
+        assert torch.equal(OF.paged_attention_chunk(**{**case, "q": other}), want)
+
+
+@pytest.mark.gpu
+def test_attention_in_a_cache_past_32_bits():
+    """Pages whose elements and bytes lie past 2^31 and 2^32."""
+    case = make(8, 8, 128, 16, [5, 1], [40, 100], device="cuda")
+    small = case["key_cache"].shape[0]
+    pages = 2 ** 32 // (16 * 8 * 128 * 2) + small
+    far = {n: torch.empty(pages, 16, 8, 128, dtype=torch.bfloat16, device="cuda")
+           for n in ("key_cache", "value_cache")}
+    for n, c in far.items():
+        c[pages - small:] = case[n]
+    tables = case["block_tables"]
+    moved = torch.where(tables < small, tables + (pages - small), tables)
+    got = OF.paged_attention_chunk(**{**case, **far, "block_tables": moved})
+    assert torch.equal(got, OF.paged_attention_chunk(**case))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("new,cached", [([1], [5000]), ([40, 1], [30, 600]), ([300], [0])])
+def test_captured_step(new, cached):
+    """Slots, cache write and attention in one graph, replayed with other lengths
+    on a stream of its own; every replay against the same calls made eagerly."""
+    heads, kv, dim, block, n = 14, 2, 64, 16, len(new)
+    case = make(heads, kv, dim, block, new, cached, device="cuda", stale=0.25)
+    rows, q = sum(new), case["q"]
+    width = case["block_tables"].shape[1]
+    spare = n * width
+    cache = [torch.randn(spare + 1, block, kv, dim, device="cuda").to(torch.bfloat16) for _ in "kv"]
+    first = torch.arange(spare, dtype=torch.int32, device="cuda").view(n, width)
+    pages = torch.tensor([spare], dtype=torch.int32, device="cuda")
+    k, v = (torch.randn(rows, kv, dim, device="cuda").to(torch.bfloat16) for _ in "kv")
+    ctx = torch.tensor(cached, dtype=torch.int32, device="cuda")
+    lens = torch.tensor(new, dtype=torch.int32, device="cuda")
+    held = torch.full((n,), width, dtype=torch.int32, device="cuda")
+
+    def step(tables, key, value):
+        plan = OF.chunk_slots(tables, ctx, lens, pages, block, rows, held)
+        OF.kv_cache_scatter(k, v, key, value, plan.slots)
+        return OF.paged_attention_chunk(q, key, value, tables, plan.cu, plan.context_lens,
+                                        dim ** -0.5, max(new))
+
+    caches = [c.clone() for c in cache]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.no_grad(), torch.cuda.stream(side):
+        step(first, *caches)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            got = step(first, *caches)
+    torch.cuda.synchronize()
+    for turn in range(4):
+        for c, x in zip(caches, cache):
+            c.copy_(x)
+        lens.copy_(torch.tensor([max(0, x - turn) for x in new]))
+        ctx.copy_(torch.tensor([max(0, x - 17 * turn) for x in cached]))
+        q.normal_()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        with torch.no_grad():
+            want = step(first.clone(), *[c.clone() for c in cache])
+        assert torch.equal(got, want), turn
+
+
+def misuse(case):
+    yield "no key before a row", {"context_lens": torch.tensor([2, 0], dtype=torch.int32)}
+    yield "table ends early", {"block_tables": case["block_tables"][:, :1].contiguous()}
+    bad = case["block_tables"].clone()
+    bad[0, 0], bad[1, 0] = -1, case["key_cache"].shape[0]
+    yield "pages outside", {"block_tables": bad}
+    yield "rows of no sequence", {"cu": torch.tensor([0, 3, 7], dtype=torch.int32)}
+    yield "rows before the first", {"cu": torch.tensor([2, 6, 9], dtype=torch.int32)}
+    yield "no table", {"block_tables": case["block_tables"][:, :0].contiguous()}
+
+
+def check_misuse(device, dtype, dim):
+    case = make(8, 2, dim, 16, [4, 5], [20, 0], device=device, dtype=dtype, spare=0, stale=0.5)
+    for name, change in misuse(case):
+        one = {**case, **{k: v.to(device) for k, v in change.items()}}
+        check(one, OF.paged_attention_chunk(**one))
+
+
+def test_pages_and_lengths_that_do_not_fit_cpu():
+    check_misuse("cpu", torch.float32, 16)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim", [64, 128])
+def test_pages_and_lengths_that_do_not_fit(dim):
+    check_misuse("cuda", torch.bfloat16, dim)
+
+
+# ------------------------------------------------------------------ slots
+
+def slots_exact(tables, ctx, new, pages, block, rows, held=None):
+    """Token by token, in Python's integers."""
+    tables, pages = [list(t) for t in tables], list(pages)
+    width = len(tables[0]) if tables else 0
+    cu, where = [0], []
+    for b, (c, n) in enumerate(zip(ctx, new)):
+        p = -(-c // block) if held is None else held[b]
+        while p * block < c + n:
+            page = pages.pop(0) if pages else -1
+            if p < width:
+                tables[b][p] = page
+            p += 1
+        for at in range(c, c + n):
+            page = tables[b][at // block] if at // block < width else -1
+            where.append((at, page * block + at % block if page >= 0 else -1))
+        cu.append(cu[-1] + n)
+    where = (where + [(0, -1)] * rows)[:rows]
+    return dict(positions=[w[0] for w in where], slots=[w[1] for w in where],
+                cu=[min(c, rows) for c in cu], context_lens=[c + n for c, n in zip(ctx, new)],
+                last=[min(max(c, 1), max(rows, 1)) - 1 for c in cu[1:]]), tables
+
+
+def check_slots(device, ctx, new, block, rows=None, held=None, width=None, free=None, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    have = [-(-c // block) for c in ctx] if held is None else held
+    need = [max(0, -(-(c + n) // block) - h) for c, n, h in zip(ctx, new, have)]
+    if width is None:
+        width = max([h + n for h, n in zip(have, need)] + [1]) + 1
+    order = torch.randperm(len(ctx) * width + sum(need) + 1, generator=g).tolist()
+    tables = [[order.pop() if i < h else -7 for i in range(width)] for h in have]
+    pages = [order.pop() for _ in range(sum(need) if free is None else free)]
+    rows = sum(new) if rows is None else rows
+    want, want_tables = slots_exact(tables, ctx, new, pages, block, rows, held)
+
+    def t(x):
+        return torch.tensor(x, dtype=torch.int32, device=device)
+
+    got_tables = t(tables).view(len(ctx), width)
+    got = OF.chunk_slots(got_tables, t(ctx), t(new), t(pages), block, rows,
+                         None if held is None else t(held))
+    for name, value in want.items():
+        assert getattr(got, name).tolist() == value, name
+    assert got_tables.tolist() == want_tables
+
+
+def slots_cases():
+    yield dict(ctx=[0], new=[1], block=16)
+    yield dict(ctx=[16], new=[1], block=16)
+    yield dict(ctx=[15], new=[1], block=16)
+    yield dict(ctx=[15, 0, 33], new=[2, 0, 100], block=16)
+    yield dict(ctx=[5, 0, 9], new=[0, 0, 0], block=4)
+    yield dict(ctx=[5, 7], new=[9, 3], block=1)
+    yield dict(ctx=[5, 7], new=[9, 3], block=7, rows=20)           # rows of no request
+    yield dict(ctx=[5, 7], new=[9, 3], block=7, rows=5)            # fewer rows than tokens
+    yield dict(ctx=[40, 40], new=[30, 5], block=8, held=[2, 9])    # fewer and more held
+    yield dict(ctx=[10, 0], new=[30, 20], block=8, free=3)         # too few pages
+    yield dict(ctx=[10, 0], new=[30, 20], block=8, width=3)        # tables too narrow
+    yield dict(ctx=[i % 50 for i in range(300)], new=[(i * 7) % 23 for i in range(300)], block=16)
+    yield dict(ctx=[0] * 257, new=[1] * 257, block=16)
+    yield dict(ctx=[0] * 3, new=[4000, 1, 2500], block=16)
+
+
+@pytest.mark.parametrize("case", slots_cases())
+def test_slots_cpu(case):
+    check_slots("cpu", **case)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", slots_cases())
+def test_slots(case):
+    check_slots("cuda", **case)
+
+
+@pytest.mark.gpu
+def test_slots_of_many_requests():
+    check_slots("cuda", ctx=[i % 77 for i in range(8192)], new=[i % 3 for i in range(8192)],
+                block=16)
+
+
+# -------------------------------------------------------------- refusals
+
+def refusals_slots(device):
+    def t(*x):
+        return torch.tensor(x, dtype=torch.int32, device=device)
+
+    args = dict(block_tables=t(1, 2).view(1, 2), context_lens=t(3), new_lens=t(4), pages=t(5),
+                block_size=16, rows=4)
+    OF.chunk_slots(**{**args, "block_tables": args["block_tables"].clone()})
+    for change in (dict(block_tables=args["block_tables"].long()), dict(context_lens=t(3, 4)),
+                   dict(new_lens=t(4).long()), dict(pages=t(5, 6)[::2].expand(2)[::2].float()),
+                   dict(block_size=0), dict(rows=-1), dict(held=t(1, 1)),
+                   dict(block_tables=t(1, 2)),
+                   dict(block_tables=t(1, 2, 3, 4).view(2, 2).t()[:1])):
+        with pytest.raises((ValueError, RuntimeError)):
+            OF.chunk_slots(**{**args, **change})
+
+
+def test_slots_refusals_cpu():
+    refusals_slots("cpu")
+
+
+@pytest.mark.gpu
+def test_slots_refusals():
+    refusals_slots("cuda")
+    n = 8193
+    with pytest.raises(RuntimeError, match="requests"):
+        z = torch.zeros(n, dtype=torch.int32, device="cuda")
+        OF.chunk_slots(z.view(n, 1), z, z, z, 16, 0)
+
+
+def test_attention_has_no_gradient():
+    case = make(4, 2, 16, 4, [3], [2], dtype=torch.float32)
+    case["q"] = case["q"].clone().requires_grad_()
+    with pytest.raises(RuntimeError, match="gradient"):
+        OF.paged_attention_chunk(**case)
+    with torch.no_grad():
+        OF.paged_attention_chunk(**case)
+        for change in (dict(scale=0.0), dict(scale=math.nan), dict(longest=-1)):
+            with pytest.raises(ValueError):
+                OF.paged_attention_chunk(**{**case, **change})
+
+
+@pytest.mark.gpu
+def test_attention_refusals():
+    case = make(8, 2, 64, 16, [4, 5], [20, 0], device="cuda")
+    good = OF.paged_attention_chunk(**case)
+    assert good.dtype == torch.bfloat16 and good.shape == case["q"].shape
+    other = make(8, 2, 64, 16, [4, 5], [20, 0], device="cuda", dtype=torch.float32)
+    key = case["key_cache"]
+    for change in (dict(q=other["q"]), dict(key_cache=other["key_cache"]),
+                   dict(q=case["q"][:, :7]), dict(q=case["q"][..., :32]),
+                   dict(key_cache=key[:, ::2]), dict(value_cache=key[:1]),
+                   dict(key_cache=key.cpu()), dict(cu=case["cu"][:2]),
+                   dict(context_lens=case["context_lens"][:1]),
+                   dict(block_tables=case["block_tables"][0]), dict(scale=0.0),
+                   dict(scale=-1.0), dict(scale=math.inf), dict(scale=math.nan),
+                   dict(longest=-1)):
+        with pytest.raises((RuntimeError, ValueError)):
+            OF.paged_attention_chunk(**{**case, **change})
