@@ -9,7 +9,15 @@
 // A workgroup owns a kv head and a block of rows that are (token, query head of the
 // group) pairs, tokens outermost: K and V are read once for all heads of the group, and a
 // block ends few tokens behind its first, so that little of the diagonal is computed in
-// vain. Products and softmax are those of the learner's attention (attention_tiles.h).
+// vain. Products and softmax are those of the learner's attention (attention_tiles.h), but
+// a wave's next scores are formed beside its weights, and K and V go into LDS by loads
+// that take no registers and stay three blocks ahead.
+//
+// 2 x 4096 behind 8192, 64/8 heads of 128 2611 us = 1053 TFLOP/s (a product of 8192^3
+// 1296), where the matrix cores are busy half of the time: a SIMD's two waves have 512
+// cycles of products and 620 of vector work a block, and little of one's hides behind the
+// other's. K and V in registers on their way to LDS, a block ahead, took 3192, 64 rows a
+// wave (one wave a SIMD) 3755, priorities of waves even.
 #include <torch/extension.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -17,8 +25,22 @@
 
 namespace {
 
-constexpr int KEYS = 64;        // of a tile
+constexpr int KEYS = 32, RING = 4;      // of a block, and blocks in LDS
+constexpr int AHEAD = 1024;             // keys whose cache rows are looked up at once
 constexpr int LEAST = 256;      // keys of a slice, at least
+
+// x / n for 0 <= x < 2^30 as a product: ceil(2^(31 + shift) / n), shift = ceil(log2(n)), is
+// too large by less than 1 and x times that less than 2^(31 + shift), so the result is exact.
+struct Divisor {
+  int n;
+  uint32_t inverse;
+  int shift;
+  Divisor(int64_t n = 1) : n((int)n), shift(0) {
+    while ((1ll << shift) < n) ++shift;
+    inverse = (uint32_t)(((1ull << (31 + shift)) + n - 1) / n);
+  }
+  DEV_INLINE int of(int x) const { return (int)(__umulhi(2u * x, inverse) >> shift); }
+};
 
 struct Chunk {
   const __hip_bfloat16* q;      // (T, H, D), heads and rows these elements apart
@@ -27,29 +49,41 @@ struct Chunk {
   const int *tables, *cu, *ctx;         // (B, width), (B + 1), (B)
   __hip_bfloat16* out;                  // (T, H, D)
   float *o_part, *ml_part;              // (slices, T, H, D), (slices, T, H, 2)
-  int T, B, H, KV, width, pages, block, shift;
+  unsigned long long *there, tag;       // (workgroups of a slice, slices), or null: another launch joins
+  int T, B, H, KV, width, pages, block;
+  Divisor by_block, by_group;           // group: query heads of a kv head
   float scale_log2;
 
   DEV_INLINE int first(int b) const { return min(max(cu[b], 0), T); }
 };
 
-// The sequence whose rows block `s` of the launch holds. Sequence b's blocks start at
-// floor(cu[b] G / ROWS) + b: as many as it may need and no sum over those before it.
-template <int ROWS>
-DEV_INLINE int start_of(const Chunk& a, int b, int group) { return a.first(b) * group / ROWS + b; }
+// The sequence whose rows block `s` of the launch holds: its first row, end and keys, its
+// number, and the block it starts at. Sequence b starts at block floor(cu[b] G / ROWS) + b:
+// as many as it may need and no sum over those before it.
+struct Sequence { int b, first, end, ctx, start; };
 
 template <int ROWS>
-DEV_INLINE int sequence_of(const Chunk& a, int s, int group) {
+DEV_INLINE int start_of(const Chunk& a, int row, int b) { return row * a.by_group.n / ROWS + b; }
+
+template <int ROWS>
+DEV_INLINE Sequence sequence_of(const Chunk& a, int s) {
   const int lane = threadIdx.x & 63;
   int lo = 0, n = a.B;
-  while (n > 1) {               // 64 candidates a turn
-    const int step = (n + 63) / 64, b = lane * step;
-    const bool before = b < n && start_of<ROWS>(a, lo + b, group) <= s;
+  while (n > 64) {              // 64 candidates a turn
+    const int step = (n + 63) / 64, i = lane * step;
+    const bool before = i < n && start_of<ROWS>(a, a.first(lo + i), lo + i) <= s;
     const int k = max(1, (int)__popcll(__ballot(before)));
     lo += (k - 1) * step;
     n = min(step, n - (k - 1) * step);
   }
-  return lo;
+  // of the last 64 all that is wanted is on its way at once: one behind the other the
+  // three numbers are a microsecond each
+  const int b = lo + min(lane, n - 1);
+  const int first = a.first(b), end = a.first(b + 1), ctx = a.ctx[b];
+  const int start = start_of<ROWS>(a, first, b);
+  const int k = max(1, (int)__popcll(__ballot(lane < n && start <= s))) - 1;
+  return {lo + k, __builtin_amdgcn_readlane(first, k), __builtin_amdgcn_readlane(end, k),
+          __builtin_amdgcn_readlane(ctx, k), __builtin_amdgcn_readlane(start, k)};
 }
 
 // Rows that no sequence has are zeros: of this kv head, by workgroup `mine` of `all`.
@@ -64,84 +98,180 @@ DEV_INLINE void clear_rows(const Chunk& a, int kv, int group, int mine, int all)
   }
 }
 
-// Rows of K and V of a tile, which lie on pages: fetched into registers, then stored to
-// LDS. Rows past the end and pages that are none read as zeros.
-template <int D, int NT>
-struct Paged {
-  static constexpr int UN = D / 8, STEP = NT / UN, PER = KEYS / STEP;
-  u32x4 k[PER], v[PER];
-  int page[PER];                // of the rows that are fetched next
-  int there;                    // a bit a row: k and v hold it
+template <typename T>
+using LDS = __attribute__((address_space(3))) T;
+template <typename T>
+DEV_INLINE LDS<T>* at(uint32_t lds) { return (LDS<T>*)(uintptr_t)lds; }
 
-  DEV_INLINE static int row(int i) { return i * STEP + threadIdx.x / UN; }
-
-  DEV_INLINE void look(const Chunk& a, const int* table, int at, int end) {
+// Addresses of a block's fragments, in registers: which block it is goes into the
+// instructions' offsets.
+template <int D>
+struct Places {
+  uint32_t row, lo[D / 32], hi[D / 32];
+  DEV_INLINE explicit Places(uint32_t lds) {
+    const Frags<D> f;
+    keep(row = lds + f.row_off);        // lds ends on 256 bytes
     #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const int j = min(at + row(i), end - 1);
-      page[i] = table[a.shift >= 0 ? j >> a.shift : j / a.block];
+    for (int dt = 0; dt < D / 32; ++dt) {
+      keep(lo[dt] = lds + (f.tr_lo ^ (dt << 6)));
+      keep(hi[dt] = lds + (f.tr_hi ^ (dt << 6)));
     }
   }
-  DEV_INLINE void fetch(const Chunk& a, int kv, int at, int end) {
-    there = 0;
-    #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const int j = at + row(i);
-      const bool ok = j < end && (unsigned)page[i] < (unsigned)a.pages;
-      const int in = a.shift >= 0 ? j & (a.block - 1) : j % a.block;
-      const int64_t off = ((int64_t)(ok ? page[i] * a.block + in : 0) * a.KV + kv) * D +
-                          threadIdx.x % UN * 8;
-      there |= (int)ok << i;
-      k[i] = *reinterpret_cast<const u32x4*>(a.key + off);
-      v[i] = *reinterpret_cast<const u32x4*>(a.value + off);
-    }
-  }
-  DEV_INLINE void store(char* kt, char* vt) {
-    if (__any(there != (1 << PER) - 1)) {
-      #pragma unroll
-      for (int i = 0; i < PER; ++i)
-        if (!(there >> i & 1)) k[i] = v[i] = u32x4{0, 0, 0, 0};
-    }
-    #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const int at = row(i) * (2 * D) + ((threadIdx.x % UN ^ swz<D>(row(i))) << 4);
-      *reinterpret_cast<u32x4*>(kt + at) = k[i];
-      *reinterpret_cast<u32x4*>(vt + at) = v[i];
-    }
+  DEV_INLINE static void keep(uint32_t& x) { asm volatile("" : "+v"(x)); }
+  DEV_INLINE bf16v8 keys(uint32_t block, int ks) const { return *at<bf16v8>((row ^ (ks << 5)) + block); }
+  DEV_INLINE bf16v8 values(uint32_t block, int k0, int dt) const {
+    const bf16v4 a = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(at<bf16v4>(lo[dt] + block + k0 * (2 * D)));
+    const bf16v4 b = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(at<bf16v4>(hi[dt] + block + k0 * (2 * D)));
+    return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
   }
 };
 
+// Not to be moved behind what follows
+DEV_INLINE void hold(bf16v8& x) {
+  u32x4 w = __builtin_bit_cast(u32x4, x);
+  asm volatile("" : "+v"(w));
+  x = __builtin_bit_cast(bf16v8, w);
+}
+
+// x + the sum of eight
+DEV_INLINE float pair_sum(const bf16v8& v, float x) {
+  const bf16v2 ones = {(__bf16)1.f, (__bf16)1.f};
+  #pragma unroll
+  for (int j = 0; j < 8; j += 2) x = __builtin_amdgcn_fdot2_f32_bf16(bf16v2{v[j], v[j + 1]}, ones, x, false);
+  return x;
+}
+
+// 16 B a lane from `from` into LDS at lds + 16 * lane. m0 is lost to the compiler, which
+// warns that nothing keeps it: nothing has to.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+DEV_INLINE void load_to_lds(uint32_t lds, uint64_t from) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
+               :: "s"(lds), "v"(from) : "m0");
+}
+#pragma clang diagnostic pop
+// Until at most VM of this wave's loads are on their way and its LDS accesses are done.
+template <int VM>
+DEV_INLINE void landed() { asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" :: "n"(VM) : "memory"); }
+DEV_INLINE void meet() {
+  __builtin_amdgcn_sched_barrier(0);
+  asm volatile("s_barrier" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
+}
+
+// Rows of K and V on pages straight into LDS, a block of KEYS at a time. Which cache row a
+// key is in stands in LDS for two runs of AHEAD keys; a row that is none (past the end, or
+// its page is outside the cache) has the sign bit there and is overwritten with zeros once
+// it has landed.
+template <int D, int NW>
+struct Paged {
+  static constexpr int UN = D / 8, PER = KEYS * UN / (NW * 64);   // lanes of a row, loads of a wave
+  static_assert(PER * NW * 64 == KEYS * UN, "block does not divide");
+  static constexpr int TB = KEYS * D * 2, BYTES = 2 * RING * TB + 2 * AHEAD * 4 + 16;
+  uint32_t lds;
+  uint64_t k[PER];              // key of row 0, this lane's 16 bytes
+  uint64_t value;               // from there to the value
+  uint32_t step;                // bytes from cache row to row
+
+  DEV_INLINE int row(int n) const { return (wave_id() * PER + n) * (64 / UN) + (threadIdx.x & 63) / UN; }
+  DEV_INLINE Paged(const Chunk& a, uint32_t lds, int kv) : lds(lds), value(reinterpret_cast<uint64_t>(a.value) - reinterpret_cast<uint64_t>(a.key)),
+        step(a.KV * D * 2) {
+    #pragma unroll
+    for (int n = 0; n < PER; ++n) {
+      const int64_t off = (int64_t)kv * D + ((threadIdx.x % UN) ^ swz<D>(row(n))) * 8;
+      k[n] = reinterpret_cast<uint64_t>(a.key + off);
+    }
+  }
+  DEV_INLINE uint32_t keys(int slot) const { return lds + (slot & (RING - 1)) * TB; }
+  DEV_INLINE uint32_t values(int slot) const { return lds + (RING + (slot & (RING - 1))) * TB; }
+  DEV_INLINE LDS<int>* lines() const { return at<int>(lds + 2 * RING * TB); }
+  DEV_INLINE LDS<int>* bad() const { return lines() + 2 * AHEAD; }   // the first key on no page
+  DEV_INLINE int line(int block, int n) const { return lines()[(block * KEYS + row(n)) & (2 * AHEAD - 1)]; }
+
+  // key j's row of the cache, or the sign bit
+  DEV_INLINE static int row_of(const Chunk& a, const int* table, int j, int end) {
+    const int of = a.by_block.of(j), page = j < end ? table[of] : -1;
+    return (unsigned)page < (unsigned)a.pages ? page * a.block + j - of * a.block : (int)0x80000000;
+  }
+  // the cache rows of keys begin + from .. + AHEAD
+  template <int UNROLL>
+  DEV_INLINE void look(const Chunk& a, const int* table, int begin, int from, int end) const {
+    #pragma unroll UNROLL
+    for (int i = 0; i < AHEAD; i += NW * 64) {
+      const int x = from + i + (int)threadIdx.x, j = begin + x, row = row_of(a, table, j, end);
+      lines()[x & (2 * AHEAD - 1)] = row;
+      if ((row < 0) & (j < end)) __hip_atomic_fetch_min(bad(), j, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+    }
+  }
+  struct Lines { int of[PER]; };
+  DEV_INLINE Lines lines_of(int block) const {
+    Lines l;
+    #pragma unroll
+    for (int n = 0; n < PER; ++n) l.of[n] = line(block, n);
+    return l;
+  }
+  // the same from the table, before lines are there
+  DEV_INLINE Lines look_up(const Chunk& a, const int* table, int begin, int block, int end) const {
+    Lines l;
+    #pragma unroll
+    for (int n = 0; n < PER; ++n) l.of[n] = row_of(a, table, begin + block * KEYS + row(n), end);
+    return l;
+  }
+  DEV_INLINE void load(uint32_t to, uint64_t more, const Lines& l) const {
+    #pragma unroll
+    for (int n = 0; n < PER; ++n)
+      load_to_lds(__builtin_amdgcn_readfirstlane(to + (wave_id() * PER + n) * 1024),
+                  k[n] + more + (uint64_t)(uint32_t)(l.of[n] & 0x7fffffff) * step);
+  }
+  DEV_INLINE void load_keys(int slot, const Lines& l) const { load(keys(slot), 0, l); }
+  DEV_INLINE void load_values(int slot, const Lines& l) const { load(values(slot), value, l); }
+  // zeros for the rows that are none; this wave's have landed
+  DEV_INLINE void mend(uint32_t slot, const Lines& l) const {
+    #pragma unroll
+    for (int n = 0; n < PER; ++n)
+      if (l.of[n] < 0)
+        *at<u32x4>(slot + (wave_id() * PER + n) * 1024 + (threadIdx.x & 63) * 16) = u32x4{0, 0, 0, 0};
+  }
+};
+
+// A wave owns 32 rows. Keys come in blocks of 32 through rings of four in LDS. A turn of
+// the loop makes the weights of block i beside the products with the keys of block i + 1,
+// which wait in registers, then adds the values of block i while the keys of block i + 2
+// are read; the keys of block i + 5 and the values of i + 3 set out meanwhile.
 template <int D, int NW>
 __global__ __launch_bounds__(NW * 64, 2)
 void chunk_attn_kernel(Chunk a) {
-  constexpr int ROWS = NW * WROWS, NS = KEYS / 32, TB = KEYS * D * 2;
-  const int group = a.H / a.KV, blocks = gridDim.x / a.KV;
+  constexpr int ROWS = NW * WROWS;
+  const int group = a.by_group.n, blocks = gridDim.x / a.KV;
   const int kv = blockIdx.x % a.KV, s = blocks - 1 - blockIdx.x / a.KV;   // longest first
   const int slices = gridDim.y, z = blockIdx.y;
-  const int none = start_of<ROWS>(a, a.B, group);
+  const int none = start_of<ROWS>(a, a.first(a.B), a.B);
+  const Sequence q = sequence_of<ROWS>(a, s);
   if (s >= none) {
     if (z == 0) clear_rows<D>(a, kv, group, s - none, blocks - none);
     return;
   }
-  const int b = __builtin_amdgcn_readfirstlane(sequence_of<ROWS>(a, s, group));
-  const int row0 = a.first(b), tokens = a.first(b + 1) - row0;
-  const int block0 = (s - start_of<ROWS>(a, b, group)) * ROWS, rows = tokens * group;
+  const int block0 = (s - q.start) * ROWS, rows = (q.end - q.first) * group;
   if (block0 < 0 || block0 >= rows) return;
 
   const int wave = wave_id(), l = threadIdx.x & 63, half = l >> 5;
-  const int before = a.ctx[b] - tokens, reach = (int)min((int64_t)a.width * a.block, (int64_t)1 << 30);
-  auto keys_of = [&](int r) { return max(0, min(before + r / group + 1, reach)); };
-  const int r0 = block0 + wave * WROWS, r = r0 + (l & 31);
-  const int rr = min(r, rows - 1), t = row0 + rr / group, head = kv * group + rr % group;
-  const int mine = keys_of(rr);                                 // keys this lane's row sees
-  const int least = keys_of(min(r0, rows - 1)), most = keys_of(min(r0 + WROWS, rows) - 1);
+  const int before = q.ctx - (q.end - q.first);
+  const int reach = (int)min((int64_t)a.width * a.block, (int64_t)1 << 30);
+  auto keys_of = [&](int r) { return max(0, min(before + a.by_group.of(r) + 1, reach)); };
+  const int r0 = block0 + wave * WROWS, r = min(r0 + (l & 31), rows - 1);
+  const int t = q.first + a.by_group.of(r), head = kv * group + r - a.by_group.of(r) * group;
+  const int mine = keys_of(r);                                  // keys this lane's row sees
+  const int least = keys_of(min(r0, rows - 1));                 // that all rows of the wave see
   const int all = keys_of(min(block0 + ROWS, rows) - 1);        // of the workgroup
   // slices of the workgroup's own keys
   const int per = max(LEAST, ((all + slices - 1) / slices + KEYS - 1) / KEYS * KEYS);
   const int begin = z * per, end = min(all, begin + per);
+  const int used = max(1, (all + per - 1) / per);
+  if (a.there && z >= used) return;
 
-  extern __shared__ __attribute__((aligned(16))) char smem[];
-  const Frags<D> fr;
+  extern __shared__ __attribute__((aligned(256))) char smem[];   // all of LDS: from 0 on
+  const uint32_t lds = (uint32_t)(uintptr_t)(LDS<char>*)smem;
+  const Places<D> fr(lds);
   bf16v8 qf[D / 16];
   {
     const __hip_bfloat16* qp = a.q + t * a.q_t + head * a.q_h;
@@ -155,95 +285,202 @@ void chunk_attn_kernel(Chunk a) {
   for (int dt = 0; dt < D / 32; ++dt) acc[dt] = zero16();
 
   if (begin < end) {
-    const int* table = a.tables + (int64_t)b * a.width;
-    Paged<D, NW * 64> tile;
-    tile.look(a, table, begin, end);
-    tile.fetch(a, kv, begin, end);
-    tile.look(a, table, begin + KEYS, end);
-    tile.store(smem, smem + TB);
+    const int* table = a.tables + (int64_t)q.b * a.width;
+    const Paged<D, NW> tile(a, lds, kv);
+    constexpr int PER = Paged<D, NW>::PER;
+    auto l1 = tile.look_up(a, table, begin, 0, end), l2 = tile.look_up(a, table, begin, 1, end),
+         l3 = tile.look_up(a, table, begin, 2, end), l4 = tile.look_up(a, table, begin, 3, end),
+         l5 = tile.look_up(a, table, begin, 4, end);
+    if (threadIdx.x == 0) *tile.bad() = 0x7fffffff;
     __syncthreads();
-    int turn = 0;
-    for (int k0 = begin; k0 < end; k0 += KEYS, turn ^= 1) {
-      char *kt = smem + turn * (2 * TB), *vt = kt + TB;
-      const bool more = k0 + KEYS < end;
-      if (more) {
-        tile.fetch(a, kv, k0 + KEYS, end);
-        tile.look(a, table, k0 + 2 * KEYS, end);
+    tile.template look<AHEAD / (NW * 64)>(a, table, begin, 0, end);
+    tile.load_keys(0, l1);
+    tile.load_keys(1, l2);
+    tile.load_keys(2, l3);
+    tile.load_values(0, l1);
+    tile.load_keys(3, l4);
+    tile.load_values(1, l2);
+    landed<2 * PER>();
+    tile.mend(tile.keys(0), l1);
+    tile.mend(tile.keys(1), l2);
+    tile.mend(tile.keys(2), l3);
+    tile.mend(tile.values(0), l1);
+    landed<2 * PER>();
+    meet();
+    bf16v8 kf[D / 16];
+    auto read_keys = [&](int block) {
+      #pragma unroll
+      for (int ks = 0; ks < D / 16; ++ks) kf[ks] = fr.keys(tile.keys(block) - lds, ks);
+    };
+    auto scores = [&](f32x16& to) {
+      to = zero16();
+      #pragma unroll
+      for (int ks = 0; ks < D / 16; ++ks) to = mfma(kf[ks], qf[ks], to);
+    };
+    f32x16 s0, s1;
+    read_keys(0);
+    scores(s0);
+    read_keys(1);
+    landed<2 * PER>();
+    meet();                     // block 4's keys land where block 0's are
+    tile.load_keys(4, l5);
+    tile.load_values(2, l3);
+    l3 = l4;                    // of the values that set out next
+    l4 = l5;
+    l5 = tile.lines_of(5);      // and of the keys
+    int whole = 0;              // keys before this one all rows see, and their pages are there
+    // Block i, whose scores are st; the next one's into next.
+    auto turn = [&](int i, f32x16& st, f32x16& next) {
+      const int k0 = begin + i * KEYS;
+      // keys that not all rows see, or rows that are none in what lands by the turn's end
+      const bool careful = k0 + 4 * KEYS > whole;
+      tile.load_keys(i + 5, l5);
+      tile.load_values(i + 3, l3);
+      l3 = l4;
+      l4 = l5;
+      l5 = tile.lines_of(i + 6);
+      bf16v8 v[2][D / 32];
+      auto read_values = [&](int k2) {
+        #pragma unroll
+        for (int dt = 0; dt < D / 32; ++dt) v[k2][dt] = fr.values(tile.values(i) - lds, k2 * 16, dt);
+      };
+      read_values(0);
+      if (careful) {
+        #pragma unroll
+        for (int j = 0; j < 16; ++j)
+          if (min(mine, end) - k0 - 4 * half <= acc_row(j, 0)) st[j] = -1e30f;
       }
-      if (k0 < most && r0 < rows) {                     // wave-uniform
-        f32x16 st[NS];
+      scores(next);             // past the end of what lies there, unused
+      // The subtracted maximum is a whole number of log2 and may lag by 2^8: weights
+      // that differ by powers of two round alike, so that tiles and slices do not
+      // change the result beyond the order of fp32 sums, and sums are hardly ever rescaled.
+      float mx = st[0];
+      #pragma unroll
+      for (int j = 1; j < 16; ++j) mx = fmaxf(mx, st[j]);
+      mx = halves_max(mx) * a.scale_log2;
+      const float to = mx > m + 8.f ? ceilf(mx) : m, fall = m - to;
+      m = to;
+      #pragma unroll
+      for (int j = 0; j < 16; ++j) st[j] = __builtin_amdgcn_exp2f(st[j] * a.scale_log2 - m);
+      bf16v8 p[2] = {pack8(st, 0), pack8(st, 1)};
+      // The sum is of the rounded weights, whose errors then cancel where few weigh much (a
+      // single key's value comes out as it is), two of them an instruction.
+      float sum = pair_sum(p[0], 0.f) + pair_sum(p[1], 0.f);
+      // here, and not behind the branch
+      hold(p[0]);
+      hold(p[1]);
+      #pragma unroll
+      for (int dt = 0; dt < D / 32; ++dt) hold(v[0][dt]);
+      if (__any(fall < 0.f)) {
+        const float alpha = __builtin_amdgcn_exp2f(fall);
+        lsum *= alpha;
         #pragma unroll
-        for (int n = 0; n < NS; ++n) {
-          st[n] = zero16();
+        for (int dt = 0; dt < D / 32; ++dt)
           #pragma unroll
-          for (int ks = 0; ks < D / 16; ++ks) st[n] = mfma(fr.row(kt, n, ks), qf[ks], st[n]);
-        }
-        if (k0 + KEYS > least) {                        // the diagonal, or the end
-          #pragma unroll
-          for (int n = 0; n < NS; ++n)
-            #pragma unroll
-            for (int i = 0; i < 16; ++i)
-              if (k0 + n * 32 + acc_row(i, half) >= mine) st[n][i] = -1e30f;
-        }
-        float mx = st[0][0];
-        #pragma unroll
-        for (int n = 0; n < NS; ++n)
-          #pragma unroll
-          for (int i = 0; i < 16; ++i) mx = fmaxf(mx, st[n][i]);
-        const float m_new = fmaxf(m, halves_max(mx) * a.scale_log2);
-        if (__any(m_new > m)) {
-          const float alpha = __builtin_amdgcn_exp2f(m - m_new);
-          lsum *= alpha;
-          #pragma unroll
-          for (int dt = 0; dt < D / 32; ++dt)
-            #pragma unroll
-            for (int i = 0; i < 16; ++i) acc[dt][i] *= alpha;
-          m = m_new;
-        }
-        #pragma unroll
-        for (int n = 0; n < NS; ++n)
-          #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            st[n][i] = __builtin_amdgcn_exp2f(st[n][i] * a.scale_log2 - m);
-            lsum += st[n][i];
-          }
-        #pragma unroll
-        for (int n = 0; n < NS; ++n)
-          #pragma unroll
-          for (int k2 = 0; k2 < 2; ++k2) {
-            const bf16v8 p = pack8(st[n], k2);
-            #pragma unroll
-            for (int dt = 0; dt < D / 32; ++dt)
-              acc[dt] = mfma(fr.col(vt, n * 32 + k2 * 16, dt), p, acc[dt]);
-          }
+          for (int j = 0; j < 16; ++j) acc[dt][j] *= alpha;
       }
-      if (more) {
-        char* next = smem + (turn ^ 1) * (2 * TB);
-        tile.store(next, next + TB);
-        __syncthreads();
+      lsum += sum;
+      read_values(1);
+      read_keys(i + 2);
+      #pragma unroll
+      for (int k2 = 0; k2 < 2; ++k2)
+        #pragma unroll
+        for (int dt = 0; dt < D / 32; ++dt) acc[dt] = mfma(v[k2][dt], p[k2], acc[dt]);
+      landed<4 * PER>();
+      if (careful) {
+        tile.mend(tile.keys(i + 3), tile.lines_of(i + 3));
+        tile.mend(tile.values(i + 1), tile.lines_of(i + 1));
+        landed<4 * PER>();
       }
+      meet();
+    };
+    for (int i = 0; begin + i * KEYS < end; i += 2) {   // an even number: the last may be empty
+      // the next run of cache rows, of which the last turns look past the end
+      if (i % (AHEAD / KEYS) == AHEAD / KEYS / 2) {
+        const int from = i * KEYS + AHEAD / 2;
+        if (begin + from < end + 8 * KEYS) tile.template look<1>(a, table, begin, from, end);
+      }
+      whole = min(min(least, end), __builtin_amdgcn_readfirstlane(*tile.bad()));
+      turn(i, s0, s1);
+      turn(i + 1, s1, s0);
     }
+    landed<0>();                        // nothing may land in LDS that is another's
   }
 
-  const bool live = r < rows, seen = mine > begin;      // else no key of this slice
+  const bool live = r0 + (l & 31) < rows, seen = mine > begin;
   lsum = halves_sum(lsum);
   if (__any(!seen)) {           // what its masked scores became is no number
     lsum = seen ? lsum : 0.f;
     #pragma unroll
     for (int dt = 0; dt < D / 32; ++dt)
       #pragma unroll
-      for (int i = 0; i < 16; ++i) acc[dt][i] = seen ? acc[dt][i] : 0.f;
+      for (int j = 0; j < 16; ++j) acc[dt][j] = seen ? acc[dt][j] : 0.f;
   }
-  const int64_t at = (int64_t)t * a.H + head;
-  if (slices == 1) {
-    store_rows<D>(acc, seen ? 1.f / lsum : 0.f, a.out + at * D, live);
+  const int64_t out = (int64_t)t * a.H + head, step = (int64_t)a.T * a.H;
+  if (slices == 1 || (a.there && used == 1)) {
+    store_rows<D>(acc, seen ? 1.f / lsum : 0.f, a.out + out * D, live);
     return;
   }
-  const int64_t part = z * (int64_t)a.T * a.H + at;
-  if (begin < end) store_rows_f32<D>(acc, a.o_part + part * D, live);
-  if (half == 0 && live) {
-    a.ml_part[part * 2] = seen ? m : -1e30f;
-    a.ml_part[part * 2 + 1] = lsum;
+  const int64_t part = z * step + out;
+  if (!a.there) {
+    if (begin < end) store_rows_f32<D>(acc, a.o_part + part * D, live);
+    if (half == 0 && live) {
+      a.ml_part[part * 2] = seen ? m : -1e30f;
+      a.ml_part[part * 2 + 1] = lsum;
+    }
+    return;
+  }
+  // the last slice of the block to end joins them
+  if (live) {
+    #pragma unroll
+    for (int dt = 0; dt < D / 32; ++dt)
+      #pragma unroll
+      for (int j = 0; j < 16; j += 2)
+        store_pair(a.o_part + part * D + dt * 32 + acc_row(j, half), acc[dt][j], acc[dt][j + 1]);
+    if (half == 0) store_pair(a.ml_part + part * 2, seen ? m : -1e30f, lsum);
+  }
+  stores_done();
+  __syncthreads();
+  int* last = reinterpret_cast<int*>(smem);
+  if (wave == 0) {
+    const bool whole = all_there(a.there + (int64_t)blockIdx.x * slices, used, z, a.tag);
+    if (l == 0) *last = whole;
+  }
+  __syncthreads();
+  if (!*last) return;
+  for (int i = threadIdx.x; i < min(ROWS, rows - block0) * (D / 4); i += NW * 64) {
+    const int row = block0 + i / (D / 4), d = i % (D / 4) * 4, of = a.by_group.of(row);
+    const int64_t at = (int64_t)(q.first + of) * a.H + kv * group + row - of * group;
+    float top = -1e30f, total = 0.f;
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+    for (int z0 = 0; z0 < used; z0 += 4) {
+      float2 ml[4], lo[4], hi[4];
+      #pragma unroll
+      for (int j = 0; j < 4; ++j) {     // past the last the last again, of no weight
+        const int64_t from = min(z0 + j, used - 1) * step + at;
+        ml[j] = load_pair(a.ml_part + from * 2);
+        lo[j] = load_pair(a.o_part + from * D + d);
+        hi[j] = load_pair(a.o_part + from * D + d + 2);
+      }
+      float high = top;
+      #pragma unroll
+      for (int j = 0; j < 4; ++j) high = fmaxf(high, ml[j].x);
+      const float old = __builtin_amdgcn_exp2f(top - high);
+      total *= old;
+      o *= old;
+      top = high;
+      #pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float f = z0 + j < used ? __builtin_amdgcn_exp2f(ml[j].x - top) : 0.f;
+        total += f * ml[j].y;
+        o += f * f32x4{lo[j].x, lo[j].y, hi[j].x, hi[j].y};
+      }
+    }
+    const float inv = total > 0.f ? 1.f / total : 0.f;
+    bf16v4 y;
+    #pragma unroll
+    for (int j = 0; j < 4; ++j) y[j] = (__bf16)(o[j] * inv);
+    *reinterpret_cast<bf16v4*>(a.out + at * D + d) = y;
   }
 }
 
@@ -339,34 +576,56 @@ torch::Tensor paged_attention_chunk(torch::Tensor q, torch::Tensor kcache, torch
   a.width = width;
   a.pages = kcache.size(0);
   a.block = block;
-  a.shift = (block & (block - 1)) == 0 ? __builtin_ctzll(block) : -1;
+  a.by_block = Divisor(block);
+  a.by_group = Divisor(H / KV);
   a.scale_log2 = (float)scale * LOG2E;
-  constexpr int NW = 4, ROWS = NW * WROWS;
   // one block more than the sequences can have, which clears the rows of none
-  const int64_t blocks = T * (H / KV) / ROWS + B + 1, grid = blocks * KV;
-  TORCH_CHECK(grid < (1ll << 31), "paged_attention_chunk: too many rows");
-  const int64_t most = width * block;
-  const int slices = (int)std::max<int64_t>(1, std::min<int64_t>({512 / grid, (most + LEAST - 1) / LEAST, 64}));
-  torch::Tensor part, ml;
-  if (slices > 1) {
-    part = torch::empty({slices, T, H, D}, q.options().dtype(at::kFloat));
-    ml = torch::empty({slices, T, H, 2}, part.options());
-    a.o_part = part.data_ptr<float>();
-    a.ml_part = ml.data_ptr<float>();
-  }
+  auto grid_of = [&](int64_t rows) { return (T * (H / KV) / rows + B + 1) * KV; };
+  const int64_t most = width * block;           // keys at most
   auto stream = at::cuda::getCurrentCUDAStream();
-  auto go = [&](auto d_) {
-    constexpr int DIM = decltype(d_)::value;
-    hipLaunchKernelGGL((chunk_attn_kernel<DIM, NW>), dim3(grid, slices), dim3(NW * 64),
-                       4 * KEYS * DIM * 2, stream, a);
-    HIP_CHECK_LAST();
+  auto go = [&](auto d_, auto nw_) {
+    constexpr int DIM = decltype(d_)::value, NW = decltype(nw_)::value;
+    const int64_t grid = grid_of(NW * WROWS);
+    TORCH_CHECK(grid < (1ll << 31), "paged_attention_chunk: too many rows");
+    // slices where the workgroups leave CUs idle: two of four waves a CU
+    const int slices = NW == 8 ? 1 : (int)std::max<int64_t>(
+        1, std::min<int64_t>({512 / grid, (most + LEAST - 1) / LEAST, 64}));
+    // Few rows are joined by the workgroups themselves: 6 single tokens of 20 to 32
+    // thousand, 40/8 heads 133.8 us with another launch, 130.0 so; 126 rows in two slices
+    // a workgroup 62 and 94.
+    const bool own = std::min<int64_t>(NW * WROWS, std::min(longest, T) * (H / KV)) * slices <= 256;
+    torch::Tensor part;
     if (slices > 1) {
+      const int64_t n = slices * T * H, marks = own ? grid * slices : 0;
+      part = torch::empty({n * (D + 2) + 2 * marks}, q.options().dtype(at::kFloat));
+      a.o_part = part.data_ptr<float>();
+      a.ml_part = a.o_part + n * D;
+      if (own) a.there = reinterpret_cast<unsigned long long*>(a.ml_part + n * 2);
+      a.tag = arrival_tag();
+    }
+    constexpr int lds = Paged<DIM, NW>::BYTES;
+    static const hipError_t raised = hipFuncSetAttribute(
+        reinterpret_cast<const void*>(chunk_attn_kernel<DIM, NW>),
+        hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+    TORCH_CHECK(raised == hipSuccess, "paged_attention_chunk: LDS");
+    hipLaunchKernelGGL((chunk_attn_kernel<DIM, NW>), dim3(grid, slices), dim3(NW * 64), lds,
+                       stream, a);
+    HIP_CHECK_LAST();
+    if (slices > 1 && !own) {
       hipLaunchKernelGGL(chunk_join_kernel<DIM>, dim3(CDIV(T * H * (DIM / 8), 256)), dim3(256), 0,
                          stream, a, slices);
       HIP_CHECK_LAST();
     }
   };
-  if (D == 128) go(std::integral_constant<int, 128>{});
-  else go(std::integral_constant<int, 64>{});
+  // 256 rows a workgroup read K and V half as often, where sequences have so many and there
+  // are enough of them, and where their fuller start is made up for: 2 x 4096 behind 8192,
+  // 64/8 heads 2793 us with 128 rows, 2611 so; 2048 behind 14336, 28/4 505 and 482; 16 x
+  // 20..120 behind 1040 45.3 and 43.0; but 10 x 200..350 behind none 27.0 and 30.9, single
+  // tokens among two chunks 97 and 133.
+  const bool wide = T * (H / KV) >= 256 * B && most >= 1024 && grid_of(256) >= 160;
+  constexpr std::integral_constant<int, 4> four{};
+  if (D == 128 && wide) go(std::integral_constant<int, 128>{}, std::integral_constant<int, 8>{});
+  else if (D == 128) go(std::integral_constant<int, 128>{}, four);
+  else go(std::integral_constant<int, 64>{}, four);
   return out;
 }

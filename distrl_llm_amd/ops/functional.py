@@ -194,6 +194,9 @@ def paged_attention_chunk(q, key_cache, value_cache, block_tables, cu,
                                    context_lens, scale)
 
 
+CHUNK_REQUESTS = 8192   # most requests of one chunk_slots on the GPU
+
+
 class ChunkSlots(NamedTuple):
     positions: torch.Tensor      # (rows,) int32; 0 behind the last request
     slots: torch.Tensor          # (rows,) int64 cache rows; -1: none

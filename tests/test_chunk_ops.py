@@ -112,7 +112,9 @@ def test_attention(new, cached, heads, kv, dim, block):
 
 
 LONG = [([1], [5000]), ([1, 1], [8191, 300]), ([3, 200], [4000, 9000]), ([33], [2500]),
-        ([9, 0, 1], [0, 700, 6000])]
+        ([9, 0, 1], [0, 700, 6000]),
+        # slices of an odd number of blocks of 32 keys
+        ([1], [18300]), ([2], [9000]), ([1, 3, 1], [9700, 4000, 12345])]
 
 
 @pytest.mark.gpu
