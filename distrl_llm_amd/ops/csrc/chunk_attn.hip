@@ -9,15 +9,18 @@
 // A workgroup owns a kv head and a block of rows that are (token, query head of the
 // group) pairs, tokens outermost: K and V are read once for all heads of the group, and a
 // block ends few tokens behind its first, so that little of the diagonal is computed in
-// vain. Products and softmax are those of the learner's attention (attention_tiles.h), but
-// a wave's next scores are formed beside its weights, and K and V go into LDS by loads
-// that take no registers and stay three blocks ahead.
+// vain. Products and softmax are those of the learner's attention (attention_tiles.h). Two
+// kernels share them: a light one and one for many rows over long contexts.
 //
-// 2 x 4096 behind 8192, 64/8 heads of 128 2611 us = 1053 TFLOP/s (a product of 8192^3
+// 2 x 4096 behind 8192, 64/8 heads of 128 2711 us = 1014 TFLOP/s (a product of 8192^3
 // 1296), where the matrix cores are busy half of the time: a SIMD's two waves have 512
-// cycles of products and 620 of vector work a block, and little of one's hides behind the
-// other's. K and V in registers on their way to LDS, a block ahead, took 3192, 64 rows a
-// wave (one wave a SIMD) 3755, priorities of waves even.
+// cycles of products and 620 of vector work each a block of 32 keys, and little of one's
+// hides behind the other's. Tried there: 128 rows a workgroup 2796, the light kernel 2975,
+// 64 rows a wave (one wave a SIMD) 3755, weights used a turn later (spills) 2959,
+// priorities of waves even. 6 single tokens behind 20 to 32 thousand, 40/8 heads 126 us =
+// 4.5 TB/s, K and V read once. 16 x 20..120 behind 1040, 28/4 44 us, 10 x 200..350 behind
+// none 22: a workgroup's start (lengths, pages, rows, one behind the other) and 9 to 35
+// blocks of 0.7 us.
 #include <torch/extension.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -25,9 +28,11 @@
 
 namespace {
 
-constexpr int KEYS = 32, RING = 4;      // of a block, and blocks in LDS
+constexpr int BLOCK = 32, RING = 4;     // keys of a block of the deep kernel, blocks in LDS
 constexpr int AHEAD = 1024;             // keys whose cache rows are looked up at once
-constexpr int LEAST = 256;      // keys of a slice, at least
+constexpr int TILE = 64;        // keys of a tile
+constexpr int LEAST = 256;      // of a slice, at least
+constexpr int FEW = 16;
 
 // x / n for 0 <= x < 2^30 as a product: ceil(2^(31 + shift) / n), shift = ceil(log2(n)), is
 // too large by less than 1 and x times that less than 2^(31 + shift), so the result is exact.
@@ -49,7 +54,6 @@ struct Chunk {
   const int *tables, *cu, *ctx;         // (B, width), (B + 1), (B)
   __hip_bfloat16* out;                  // (T, H, D)
   float *o_part, *ml_part;              // (slices, T, H, D), (slices, T, H, 2)
-  unsigned long long *there, tag;       // (workgroups of a slice, slices), or null: another launch joins
   int T, B, H, KV, width, pages, block;
   Divisor by_block, by_group;           // group: query heads of a kv head
   float scale_log2;
@@ -103,6 +107,261 @@ using LDS = __attribute__((address_space(3))) T;
 template <typename T>
 DEV_INLINE LDS<T>* at(uint32_t lds) { return (LDS<T>*)(uintptr_t)lds; }
 
+// What a workgroup works on: rows block0 .. of sequence q's (token, head) pairs, and a slice
+// of the keys that its last row sees. Of those a lane's own row: token t, its head, and
+// keys; least: keys that all rows of the wave see.
+struct Work {
+  Sequence q;
+  int rows, block0, t, head, mine, least, begin, end;
+  bool live;
+};
+
+// Whether there is any work; if not, rows of no sequence have been cleared.
+template <int D, int NW>
+DEV_INLINE bool find_work(const Chunk& a, Work& w) {
+  constexpr int ROWS = NW * WROWS;
+  const int group = a.by_group.n, blocks = gridDim.x / a.KV;
+  const int kv = blockIdx.x % a.KV, s = blocks - 1 - blockIdx.x / a.KV;   // longest first
+  const int none = start_of<ROWS>(a, a.first(a.B), a.B);
+  w.q = sequence_of<ROWS>(a, s);
+  if (s >= none) {
+    if (blockIdx.y == 0) clear_rows<D>(a, kv, group, s - none, blocks - none);
+    return false;
+  }
+  w.block0 = (s - w.q.start) * ROWS;
+  w.rows = (w.q.end - w.q.first) * group;
+  if (w.block0 < 0 || w.block0 >= w.rows) return false;
+  const int before = w.q.ctx - (w.q.end - w.q.first);
+  const int reach = (int)min((int64_t)a.width * a.block, (int64_t)1 << 30);
+  auto keys_of = [&](int r) { return max(0, min(before + a.by_group.of(r) + 1, reach)); };
+  const int r0 = w.block0 + wave_id() * WROWS, row = r0 + (threadIdx.x & 31);
+  const int r = min(row, w.rows - 1), of = a.by_group.of(r);
+  w.live = row < w.rows;
+  w.t = w.q.first + of;
+  w.head = kv * group + r - of * group;
+  w.mine = keys_of(r);
+  w.least = keys_of(min(r0, w.rows - 1));
+  const int all = keys_of(min(w.block0 + ROWS, w.rows) - 1), slices = gridDim.y;
+  const int per = max(LEAST, ((all + slices - 1) / slices + TILE - 1) / TILE * TILE);
+  w.begin = blockIdx.y * per;
+  w.end = min(all, w.begin + per);
+  return true;
+}
+
+template <int D>
+DEV_INLINE void load_queries(const Chunk& a, const Work& w, bf16v8 (&qf)[D / 16]) {
+  const __hip_bfloat16* qp = a.q + w.t * a.q_t + w.head * a.q_h + ((threadIdx.x & 63) >> 5) * 8;
+  #pragma unroll
+  for (int ks = 0; ks < D / 16; ++ks) qf[ks] = *reinterpret_cast<const bf16v8*>(qp + ks * 16);
+}
+
+// Scores of keys that this lane's row does not see; k0: the first
+DEV_INLINE void hide(f32x16& st, const Work& w, int k0) {
+  const int seen = min(w.mine, w.end) - k0 - 4 * ((int)(threadIdx.x & 63) >> 5);
+  #pragma unroll
+  for (int j = 0; j < 16; ++j)
+    if (seen <= acc_row(j, 0)) st[j] = -1e30f;
+}
+
+// x + the sum of eight
+DEV_INLINE float pair_sum(const bf16v8& v, float x) {
+  const bf16v2 ones = {(__bf16)1.f, (__bf16)1.f};
+  #pragma unroll
+  for (int j = 0; j < 8; j += 2) x = __builtin_amdgcn_fdot2_f32_bf16(bf16v2{v[j], v[j + 1]}, ones, x, false);
+  return x;
+}
+
+// Scores into weights p, which carry 2^-m of their own, and their sum; what m moved by is
+// returned, and what was weighed before is to be rescaled by 2 to that.
+// m is a whole number and may lag by 8: weights that differ by powers of two round alike,
+// so that tiles and slices do not change the result beyond the order of fp32 sums, and
+// sums are hardly ever rescaled. The sum is of the weights before they are rounded, whose
+// errors are even; of rows that see 16 keys at most (few) it is of the rounded ones, whose
+// errors cancel then (a single key's value comes out as it is).
+template <int NS>
+DEV_INLINE float weigh(f32x16 (&st)[NS], bf16v8 (&p)[NS][2], float& m, float& sum, bool few,
+                       float scale_log2) {
+  float mx = st[0][0];
+  #pragma unroll
+  for (int n = 0; n < NS; ++n)
+    #pragma unroll
+    for (int j = 0; j < 16; ++j) mx = fmaxf(mx, st[n][j]);
+  mx = halves_max(mx) * scale_log2;
+  const float to = mx > m + 8.f ? ceilf(mx) : m, fall = m - to;
+  m = to;
+  sum = 0.f;
+  #pragma unroll
+  for (int n = 0; n < NS; ++n) {
+    #pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      st[n][j] = __builtin_amdgcn_exp2f(st[n][j] * scale_log2 - m);
+      sum += st[n][j];
+    }
+    #pragma unroll
+    for (int k2 = 0; k2 < 2; ++k2) p[n][k2] = pack8(st[n], k2);
+  }
+  if (__any(few)) {
+    float rounded = 0.f;
+    #pragma unroll
+    for (int n = 0; n < NS; ++n)
+      #pragma unroll
+      for (int k2 = 0; k2 < 2; ++k2) rounded = pair_sum(p[n][k2], rounded);
+    sum = few ? rounded : sum;
+  }
+  return fall;
+}
+
+template <int D>
+DEV_INLINE void rescale(float fall, float& lsum, f32x16 (&acc)[D / 32]) {
+  const float alpha = __builtin_amdgcn_exp2f(fall);
+  lsum *= alpha;
+  #pragma unroll
+  for (int dt = 0; dt < D / 32; ++dt)
+    #pragma unroll
+    for (int j = 0; j < 16; ++j) acc[dt][j] *= alpha;
+}
+
+// This lane's row, or its part of it, into memory.
+template <int D>
+DEV_INLINE void finish(const Chunk& a, const Work& w, float m, float lsum, f32x16 (&acc)[D / 32]) {
+  const bool seen = w.mine > w.begin;
+  lsum = halves_sum(lsum);
+  if (__any(!seen)) {           // what its masked scores became is no number
+    lsum = seen ? lsum : 0.f;
+    #pragma unroll
+    for (int dt = 0; dt < D / 32; ++dt)
+      #pragma unroll
+      for (int j = 0; j < 16; ++j) acc[dt][j] = seen ? acc[dt][j] : 0.f;
+  }
+  const int64_t at = (int64_t)w.t * a.H + w.head;
+  if (gridDim.y == 1) {
+    store_rows<D>(acc, seen ? 1.f / lsum : 0.f, a.out + at * D, w.live);
+    return;
+  }
+  const int64_t part = blockIdx.y * (int64_t)a.T * a.H + at;
+  if (w.begin < w.end) store_rows_f32<D>(acc, a.o_part + part * D, w.live);
+  if ((threadIdx.x & 63) < 32 && w.live) {
+    a.ml_part[part * 2] = seen ? m : -1e30f;
+    a.ml_part[part * 2 + 1] = lsum;
+  }
+}
+
+// Rows of K and V of a tile: fetched into registers, then stored to LDS. Rows
+// past the end and pages that are none read as zeros.
+template <int D, int NT>
+struct Staged {
+  static constexpr int UN = D / 8, STEP = NT / UN, PER = TILE / STEP;
+  static_assert(TILE % STEP == 0, "tile does not divide");
+  u32x4 k[PER], v[PER];
+  int page[PER];                // of the rows that are fetched next
+  int there;                    // a bit a row: k and v hold it
+
+  DEV_INLINE static int row(int i) { return i * STEP + threadIdx.x / UN; }
+
+  DEV_INLINE void look(const Chunk& a, const int* table, int at, int end) {
+    #pragma unroll
+    for (int i = 0; i < PER; ++i) page[i] = table[a.by_block.of(min(at + row(i), end - 1))];
+  }
+  DEV_INLINE void fetch(const Chunk& a, int kv, int at, int end) {
+    there = 0;
+    #pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int j = at + row(i), in = j - a.by_block.of(j) * a.block;
+      const bool ok = (j < end) & ((unsigned)page[i] < (unsigned)a.pages);
+      const int64_t off = ((int64_t)(ok ? page[i] * a.block + in : 0) * a.KV + kv) * D +
+                          threadIdx.x % UN * 8;
+      there |= (int)ok << i;
+      k[i] = *reinterpret_cast<const u32x4*>(a.key + off);
+      v[i] = *reinterpret_cast<const u32x4*>(a.value + off);
+    }
+  }
+  DEV_INLINE void store(char* kt, char* vt) {
+    if (__any(there != (1 << PER) - 1)) {
+      #pragma unroll
+      for (int i = 0; i < PER; ++i)
+        if (!(there >> i & 1)) k[i] = v[i] = u32x4{0, 0, 0, 0};
+    }
+    #pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int at = row(i) * (2 * D) + ((threadIdx.x % UN ^ swz<D>(row(i))) << 4);
+      *reinterpret_cast<u32x4*>(kt + at) = k[i];
+      *reinterpret_cast<u32x4*>(vt + at) = v[i];
+    }
+  }
+};
+
+// Shorter contexts and fewer rows: tiles of 64 keys, the next one on its way into registers
+// while this one's scores, weights and values follow one another. It starts in half the
+// time of the kernel below. (Two waves a workgroup and tiles of 32: 10 x 200..350 behind
+// none, 28/4 heads 22.7 us for 22.1, 80 x 100 33.8 for 37.4, 4 x 1200 85 for 67.)
+template <int D, int NW>
+__global__ __launch_bounds__(NW * 64, 2)
+void chunk_attn_kernel(Chunk a) {
+  constexpr int NS = TILE / 32, TB = TILE * D * 2;
+  Work w;
+  if (!find_work<D, NW>(a, w)) return;
+  const int kv = blockIdx.x % a.KV;
+  extern __shared__ __attribute__((aligned(256))) char smem[];
+  const Frags<D> fr;
+  bf16v8 qf[D / 16];
+  load_queries<D>(a, w, qf);
+  float m = -1e30f, lsum = 0.f;
+  f32x16 acc[D / 32];
+  #pragma unroll
+  for (int dt = 0; dt < D / 32; ++dt) acc[dt] = zero16();
+
+  if (w.begin < w.end) {
+    const int* table = a.tables + (int64_t)w.q.b * a.width;
+    const int most = __builtin_amdgcn_readlane(w.mine, 31);       // of the wave's rows
+    Staged<D, NW * 64> tile;
+    tile.look(a, table, w.begin, w.end);
+    tile.fetch(a, kv, w.begin, w.end);
+    tile.look(a, table, w.begin + TILE, w.end);
+    tile.store(smem, smem + TB);
+    __syncthreads();
+    int turn = 0;
+    for (int k0 = w.begin; k0 < w.end; k0 += TILE, turn ^= 1) {
+      char *kt = smem + turn * (2 * TB), *vt = kt + TB;
+      const bool more = k0 + TILE < w.end;
+      if (more) {
+        tile.fetch(a, kv, k0 + TILE, w.end);
+        tile.look(a, table, k0 + 2 * TILE, w.end);
+      }
+      if (k0 < most && w.block0 + wave_id() * WROWS < w.rows) {   // wave-uniform
+        f32x16 st[NS];
+        #pragma unroll
+        for (int n = 0; n < NS; ++n) {
+          st[n] = zero16();
+          #pragma unroll
+          for (int ks = 0; ks < D / 16; ++ks) st[n] = mfma(fr.row(kt, n, ks), qf[ks], st[n]);
+        }
+        if (k0 + TILE > min(w.least, w.end)) {          // the diagonal, or the end
+          #pragma unroll
+          for (int n = 0; n < NS; ++n) hide(st[n], w, k0 + n * 32);
+        }
+        bf16v8 p[NS][2];
+        float sum;
+        const float fall = weigh(st, p, m, sum, w.mine <= FEW, a.scale_log2);
+        if (__any(fall < 0.f)) rescale<D>(fall, lsum, acc);
+        lsum += sum;
+        #pragma unroll
+        for (int n = 0; n < NS; ++n)
+          #pragma unroll
+          for (int k2 = 0; k2 < 2; ++k2)
+            #pragma unroll
+            for (int dt = 0; dt < D / 32; ++dt)
+              acc[dt] = mfma(fr.col(vt, n * 32 + k2 * 16, dt), p[n][k2], acc[dt]);
+      }
+      if (more) {
+        char* next = smem + (turn ^ 1) * (2 * TB);
+        tile.store(next, next + TB);
+        __syncthreads();
+      }
+    }
+  }
+  finish<D>(a, w, m, lsum, acc);
+}
+
 // Addresses of a block's fragments, in registers: which block it is goes into the
 // instructions' offsets.
 template <int D>
@@ -133,14 +392,6 @@ DEV_INLINE void hold(bf16v8& x) {
   x = __builtin_bit_cast(bf16v8, w);
 }
 
-// x + the sum of eight
-DEV_INLINE float pair_sum(const bf16v8& v, float x) {
-  const bf16v2 ones = {(__bf16)1.f, (__bf16)1.f};
-  #pragma unroll
-  for (int j = 0; j < 8; j += 2) x = __builtin_amdgcn_fdot2_f32_bf16(bf16v2{v[j], v[j + 1]}, ones, x, false);
-  return x;
-}
-
 // 16 B a lane from `from` into LDS at lds + 16 * lane. m0 is lost to the compiler, which
 // warns that nothing keeps it: nothing has to.
 #pragma clang diagnostic push
@@ -159,15 +410,15 @@ DEV_INLINE void meet() {
   __builtin_amdgcn_sched_barrier(0);
 }
 
-// Rows of K and V on pages straight into LDS, a block of KEYS at a time. Which cache row a
+// Rows of K and V on pages straight into LDS, a block of BLOCK at a time. Which cache row a
 // key is in stands in LDS for two runs of AHEAD keys; a row that is none (past the end, or
 // its page is outside the cache) has the sign bit there and is overwritten with zeros once
 // it has landed.
 template <int D, int NW>
 struct Paged {
-  static constexpr int UN = D / 8, PER = KEYS * UN / (NW * 64);   // lanes of a row, loads of a wave
-  static_assert(PER * NW * 64 == KEYS * UN, "block does not divide");
-  static constexpr int TB = KEYS * D * 2, BYTES = 2 * RING * TB + 2 * AHEAD * 4 + 16;
+  static constexpr int UN = D / 8, PER = BLOCK * UN / (NW * 64);   // lanes of a row, loads of a wave
+  static_assert(PER * NW * 64 == BLOCK * UN, "block does not divide");
+  static constexpr int TB = BLOCK * D * 2, BYTES = 2 * RING * TB + 2 * AHEAD * 4 + 16;
   uint32_t lds;
   uint64_t k[PER];              // key of row 0, this lane's 16 bytes
   uint64_t value;               // from there to the value
@@ -186,7 +437,7 @@ struct Paged {
   DEV_INLINE uint32_t values(int slot) const { return lds + (RING + (slot & (RING - 1))) * TB; }
   DEV_INLINE LDS<int>* lines() const { return at<int>(lds + 2 * RING * TB); }
   DEV_INLINE LDS<int>* bad() const { return lines() + 2 * AHEAD; }   // the first key on no page
-  DEV_INLINE int line(int block, int n) const { return lines()[(block * KEYS + row(n)) & (2 * AHEAD - 1)]; }
+  DEV_INLINE int line(int block, int n) const { return lines()[(block * BLOCK + row(n)) & (2 * AHEAD - 1)]; }
 
   // key j's row of the cache, or the sign bit
   DEV_INLINE static int row_of(const Chunk& a, const int* table, int j, int end) {
@@ -214,7 +465,7 @@ struct Paged {
   DEV_INLINE Lines look_up(const Chunk& a, const int* table, int begin, int block, int end) const {
     Lines l;
     #pragma unroll
-    for (int n = 0; n < PER; ++n) l.of[n] = row_of(a, table, begin + block * KEYS + row(n), end);
+    for (int n = 0; n < PER; ++n) l.of[n] = row_of(a, table, begin + block * BLOCK + row(n), end);
     return l;
   }
   DEV_INLINE void load(uint32_t to, uint64_t more, const Lines& l) const {
@@ -234,58 +485,28 @@ struct Paged {
   }
 };
 
-// A wave owns 32 rows. Keys come in blocks of 32 through rings of four in LDS. A turn of
-// the loop makes the weights of block i beside the products with the keys of block i + 1,
+// Many rows and long contexts: keys come in blocks of 32 through rings of four in LDS. A turn of the
+// loop makes the weights of block i beside the products with the keys of block i + 1,
 // which wait in registers, then adds the values of block i while the keys of block i + 2
 // are read; the keys of block i + 5 and the values of i + 3 set out meanwhile.
 template <int D, int NW>
 __global__ __launch_bounds__(NW * 64, 2)
-void chunk_attn_kernel(Chunk a) {
-  constexpr int ROWS = NW * WROWS;
-  const int group = a.by_group.n, blocks = gridDim.x / a.KV;
-  const int kv = blockIdx.x % a.KV, s = blocks - 1 - blockIdx.x / a.KV;   // longest first
-  const int slices = gridDim.y, z = blockIdx.y;
-  const int none = start_of<ROWS>(a, a.first(a.B), a.B);
-  const Sequence q = sequence_of<ROWS>(a, s);
-  if (s >= none) {
-    if (z == 0) clear_rows<D>(a, kv, group, s - none, blocks - none);
-    return;
-  }
-  const int block0 = (s - q.start) * ROWS, rows = (q.end - q.first) * group;
-  if (block0 < 0 || block0 >= rows) return;
-
-  const int wave = wave_id(), l = threadIdx.x & 63, half = l >> 5;
-  const int before = q.ctx - (q.end - q.first);
-  const int reach = (int)min((int64_t)a.width * a.block, (int64_t)1 << 30);
-  auto keys_of = [&](int r) { return max(0, min(before + a.by_group.of(r) + 1, reach)); };
-  const int r0 = block0 + wave * WROWS, r = min(r0 + (l & 31), rows - 1);
-  const int t = q.first + a.by_group.of(r), head = kv * group + r - a.by_group.of(r) * group;
-  const int mine = keys_of(r);                                  // keys this lane's row sees
-  const int least = keys_of(min(r0, rows - 1));                 // that all rows of the wave see
-  const int all = keys_of(min(block0 + ROWS, rows) - 1);        // of the workgroup
-  // slices of the workgroup's own keys
-  const int per = max(LEAST, ((all + slices - 1) / slices + KEYS - 1) / KEYS * KEYS);
-  const int begin = z * per, end = min(all, begin + per);
-  const int used = max(1, (all + per - 1) / per);
-  if (a.there && z >= used) return;
-
+void chunk_deep_kernel(Chunk a) {
+  Work w;
+  if (!find_work<D, NW>(a, w)) return;
+  const int kv = blockIdx.x % a.KV, begin = w.begin, end = w.end;
   extern __shared__ __attribute__((aligned(256))) char smem[];   // all of LDS: from 0 on
   const uint32_t lds = (uint32_t)(uintptr_t)(LDS<char>*)smem;
   const Places<D> fr(lds);
   bf16v8 qf[D / 16];
-  {
-    const __hip_bfloat16* qp = a.q + t * a.q_t + head * a.q_h;
-    #pragma unroll
-    for (int ks = 0; ks < D / 16; ++ks)
-      qf[ks] = *reinterpret_cast<const bf16v8*>(qp + ks * 16 + half * 8);
-  }
+  load_queries<D>(a, w, qf);
   float m = -1e30f, lsum = 0.f;
   f32x16 acc[D / 32];
   #pragma unroll
   for (int dt = 0; dt < D / 32; ++dt) acc[dt] = zero16();
 
   if (begin < end) {
-    const int* table = a.tables + (int64_t)q.b * a.width;
+    const int* table = a.tables + (int64_t)w.q.b * a.width;
     const Paged<D, NW> tile(a, lds, kv);
     constexpr int PER = Paged<D, NW>::PER;
     auto l1 = tile.look_up(a, table, begin, 0, end), l2 = tile.look_up(a, table, begin, 1, end),
@@ -317,9 +538,9 @@ void chunk_attn_kernel(Chunk a) {
       #pragma unroll
       for (int ks = 0; ks < D / 16; ++ks) to = mfma(kf[ks], qf[ks], to);
     };
-    f32x16 s0, s1;
+    f32x16 s0[1], s1[1];
     read_keys(0);
-    scores(s0);
+    scores(s0[0]);
     read_keys(1);
     landed<2 * PER>();
     meet();                     // block 4's keys land where block 0's are
@@ -330,10 +551,10 @@ void chunk_attn_kernel(Chunk a) {
     l5 = tile.lines_of(5);      // and of the keys
     int whole = 0;              // keys before this one all rows see, and their pages are there
     // Block i, whose scores are st; the next one's into next.
-    auto turn = [&](int i, f32x16& st, f32x16& next) {
-      const int k0 = begin + i * KEYS;
+    auto turn = [&](int i, f32x16 (&st)[1], f32x16& next) {
+      const int k0 = begin + i * BLOCK;
       // keys that not all rows see, or rows that are none in what lands by the turn's end
-      const bool careful = k0 + 4 * KEYS > whole;
+      const bool careful = k0 + 4 * BLOCK > whole;
       tile.load_keys(i + 5, l5);
       tile.load_values(i + 3, l3);
       l3 = l4;
@@ -345,47 +566,24 @@ void chunk_attn_kernel(Chunk a) {
         for (int dt = 0; dt < D / 32; ++dt) v[k2][dt] = fr.values(tile.values(i) - lds, k2 * 16, dt);
       };
       read_values(0);
-      if (careful) {
-        #pragma unroll
-        for (int j = 0; j < 16; ++j)
-          if (min(mine, end) - k0 - 4 * half <= acc_row(j, 0)) st[j] = -1e30f;
-      }
+      if (careful) hide(st[0], w, k0);
       scores(next);             // past the end of what lies there, unused
-      // The subtracted maximum is a whole number of log2 and may lag by 2^8: weights
-      // that differ by powers of two round alike, so that tiles and slices do not
-      // change the result beyond the order of fp32 sums, and sums are hardly ever rescaled.
-      float mx = st[0];
-      #pragma unroll
-      for (int j = 1; j < 16; ++j) mx = fmaxf(mx, st[j]);
-      mx = halves_max(mx) * a.scale_log2;
-      const float to = mx > m + 8.f ? ceilf(mx) : m, fall = m - to;
-      m = to;
-      #pragma unroll
-      for (int j = 0; j < 16; ++j) st[j] = __builtin_amdgcn_exp2f(st[j] * a.scale_log2 - m);
-      bf16v8 p[2] = {pack8(st, 0), pack8(st, 1)};
-      // The sum is of the rounded weights, whose errors then cancel where few weigh much (a
-      // single key's value comes out as it is), two of them an instruction.
-      float sum = pair_sum(p[0], 0.f) + pair_sum(p[1], 0.f);
+      bf16v8 p[1][2];
+      float sum;
+      const float fall = weigh(st, p, m, sum, w.mine <= FEW, a.scale_log2);
       // here, and not behind the branch
-      hold(p[0]);
-      hold(p[1]);
+      hold(p[0][0]);
+      hold(p[0][1]);
       #pragma unroll
       for (int dt = 0; dt < D / 32; ++dt) hold(v[0][dt]);
-      if (__any(fall < 0.f)) {
-        const float alpha = __builtin_amdgcn_exp2f(fall);
-        lsum *= alpha;
-        #pragma unroll
-        for (int dt = 0; dt < D / 32; ++dt)
-          #pragma unroll
-          for (int j = 0; j < 16; ++j) acc[dt][j] *= alpha;
-      }
+      if (__any(fall < 0.f)) rescale<D>(fall, lsum, acc);
       lsum += sum;
       read_values(1);
       read_keys(i + 2);
       #pragma unroll
       for (int k2 = 0; k2 < 2; ++k2)
         #pragma unroll
-        for (int dt = 0; dt < D / 32; ++dt) acc[dt] = mfma(v[k2][dt], p[k2], acc[dt]);
+        for (int dt = 0; dt < D / 32; ++dt) acc[dt] = mfma(v[k2][dt], p[0][k2], acc[dt]);
       landed<4 * PER>();
       if (careful) {
         tile.mend(tile.keys(i + 3), tile.lines_of(i + 3));
@@ -394,94 +592,20 @@ void chunk_attn_kernel(Chunk a) {
       }
       meet();
     };
-    for (int i = 0; begin + i * KEYS < end; i += 2) {   // an even number: the last may be empty
+    for (int i = 0; begin + i * BLOCK < end; i += 2) {   // an even number: the last may be empty
       // the next run of cache rows, of which the last turns look past the end
-      if (i % (AHEAD / KEYS) == AHEAD / KEYS / 2) {
-        const int from = i * KEYS + AHEAD / 2;
-        if (begin + from < end + 8 * KEYS) tile.template look<1>(a, table, begin, from, end);
+      if (i % (AHEAD / BLOCK) == AHEAD / BLOCK / 2) {
+        const int from = i * BLOCK + AHEAD / 2;
+        if (begin + from < end + 8 * BLOCK) tile.template look<1>(a, table, begin, from, end);
       }
-      whole = min(min(least, end), __builtin_amdgcn_readfirstlane(*tile.bad()));
-      turn(i, s0, s1);
-      turn(i + 1, s1, s0);
+      whole = min(min(w.least, end), __builtin_amdgcn_readfirstlane(*tile.bad()));
+      turn(i, s0, s1[0]);
+      turn(i + 1, s1, s0[0]);
     }
     landed<0>();                        // nothing may land in LDS that is another's
   }
 
-  const bool live = r0 + (l & 31) < rows, seen = mine > begin;
-  lsum = halves_sum(lsum);
-  if (__any(!seen)) {           // what its masked scores became is no number
-    lsum = seen ? lsum : 0.f;
-    #pragma unroll
-    for (int dt = 0; dt < D / 32; ++dt)
-      #pragma unroll
-      for (int j = 0; j < 16; ++j) acc[dt][j] = seen ? acc[dt][j] : 0.f;
-  }
-  const int64_t out = (int64_t)t * a.H + head, step = (int64_t)a.T * a.H;
-  if (slices == 1 || (a.there && used == 1)) {
-    store_rows<D>(acc, seen ? 1.f / lsum : 0.f, a.out + out * D, live);
-    return;
-  }
-  const int64_t part = z * step + out;
-  if (!a.there) {
-    if (begin < end) store_rows_f32<D>(acc, a.o_part + part * D, live);
-    if (half == 0 && live) {
-      a.ml_part[part * 2] = seen ? m : -1e30f;
-      a.ml_part[part * 2 + 1] = lsum;
-    }
-    return;
-  }
-  // the last slice of the block to end joins them
-  if (live) {
-    #pragma unroll
-    for (int dt = 0; dt < D / 32; ++dt)
-      #pragma unroll
-      for (int j = 0; j < 16; j += 2)
-        store_pair(a.o_part + part * D + dt * 32 + acc_row(j, half), acc[dt][j], acc[dt][j + 1]);
-    if (half == 0) store_pair(a.ml_part + part * 2, seen ? m : -1e30f, lsum);
-  }
-  stores_done();
-  __syncthreads();
-  int* last = reinterpret_cast<int*>(smem);
-  if (wave == 0) {
-    const bool whole = all_there(a.there + (int64_t)blockIdx.x * slices, used, z, a.tag);
-    if (l == 0) *last = whole;
-  }
-  __syncthreads();
-  if (!*last) return;
-  for (int i = threadIdx.x; i < min(ROWS, rows - block0) * (D / 4); i += NW * 64) {
-    const int row = block0 + i / (D / 4), d = i % (D / 4) * 4, of = a.by_group.of(row);
-    const int64_t at = (int64_t)(q.first + of) * a.H + kv * group + row - of * group;
-    float top = -1e30f, total = 0.f;
-    f32x4 o = {0.f, 0.f, 0.f, 0.f};
-    for (int z0 = 0; z0 < used; z0 += 4) {
-      float2 ml[4], lo[4], hi[4];
-      #pragma unroll
-      for (int j = 0; j < 4; ++j) {     // past the last the last again, of no weight
-        const int64_t from = min(z0 + j, used - 1) * step + at;
-        ml[j] = load_pair(a.ml_part + from * 2);
-        lo[j] = load_pair(a.o_part + from * D + d);
-        hi[j] = load_pair(a.o_part + from * D + d + 2);
-      }
-      float high = top;
-      #pragma unroll
-      for (int j = 0; j < 4; ++j) high = fmaxf(high, ml[j].x);
-      const float old = __builtin_amdgcn_exp2f(top - high);
-      total *= old;
-      o *= old;
-      top = high;
-      #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float f = z0 + j < used ? __builtin_amdgcn_exp2f(ml[j].x - top) : 0.f;
-        total += f * ml[j].y;
-        o += f * f32x4{lo[j].x, lo[j].y, hi[j].x, hi[j].y};
-      }
-    }
-    const float inv = total > 0.f ? 1.f / total : 0.f;
-    bf16v4 y;
-    #pragma unroll
-    for (int j = 0; j < 4; ++j) y[j] = (__bf16)(o[j] * inv);
-    *reinterpret_cast<bf16v4*>(a.out + at * D + d) = y;
-  }
+  finish<D>(a, w, m, lsum, acc);
 }
 
 // The slices of a row joined; eight elements a thread.
@@ -583,49 +707,55 @@ torch::Tensor paged_attention_chunk(torch::Tensor q, torch::Tensor kcache, torch
   auto grid_of = [&](int64_t rows) { return (T * (H / KV) / rows + B + 1) * KV; };
   const int64_t most = width * block;           // keys at most
   auto stream = at::cuda::getCurrentCUDAStream();
-  auto go = [&](auto d_, auto nw_) {
-    constexpr int DIM = decltype(d_)::value, NW = decltype(nw_)::value;
-    const int64_t grid = grid_of(NW * WROWS);
+  auto check = [](int64_t grid) {
     TORCH_CHECK(grid < (1ll << 31), "paged_attention_chunk: too many rows");
-    // slices where the workgroups leave CUs idle: two of four waves a CU
-    const int slices = NW == 8 ? 1 : (int)std::max<int64_t>(
-        1, std::min<int64_t>({512 / grid, (most + LEAST - 1) / LEAST, 64}));
-    // Few rows are joined by the workgroups themselves: 6 single tokens of 20 to 32
-    // thousand, 40/8 heads 133.8 us with another launch, 130.0 so; 126 rows in two slices
-    // a workgroup 62 and 94.
-    const bool own = std::min<int64_t>(NW * WROWS, std::min(longest, T) * (H / KV)) * slices <= 256;
-    torch::Tensor part;
-    if (slices > 1) {
-      const int64_t n = slices * T * H, marks = own ? grid * slices : 0;
-      part = torch::empty({n * (D + 2) + 2 * marks}, q.options().dtype(at::kFloat));
-      a.o_part = part.data_ptr<float>();
-      a.ml_part = a.o_part + n * D;
-      if (own) a.there = reinterpret_cast<unsigned long long*>(a.ml_part + n * 2);
-      a.tag = arrival_tag();
-    }
-    constexpr int lds = Paged<DIM, NW>::BYTES;
+    return grid;
+  };
+  auto deep = [&] {
+    constexpr int DIM = 128, NW = 8, lds = Paged<DIM, NW>::BYTES;
     static const hipError_t raised = hipFuncSetAttribute(
-        reinterpret_cast<const void*>(chunk_attn_kernel<DIM, NW>),
+        reinterpret_cast<const void*>(chunk_deep_kernel<DIM, NW>),
         hipFuncAttributeMaxDynamicSharedMemorySize, lds);
     TORCH_CHECK(raised == hipSuccess, "paged_attention_chunk: LDS");
-    hipLaunchKernelGGL((chunk_attn_kernel<DIM, NW>), dim3(grid, slices), dim3(NW * 64), lds,
-                       stream, a);
+    hipLaunchKernelGGL((chunk_deep_kernel<DIM, NW>), dim3(check(grid_of(NW * WROWS))),
+                       dim3(NW * 64), lds, stream, a);
     HIP_CHECK_LAST();
-    if (slices > 1 && !own) {
+  };
+  auto light = [&](auto d_) {
+    constexpr int DIM = decltype(d_)::value, NW = 4;
+    const int64_t grid = check(grid_of(NW * WROWS));
+    // Slices where the workgroups leave CUs idle (two of four waves a CU), of 256 keys at
+    // least and from three of them on: the join is a launch of 4 us. 5 tokens behind 1040,
+    // 14/2 heads of 64 12.2 us, one slice 18.
+    const int slices = most < 3 * LEAST ? 1 : (int)std::max<int64_t>(
+        1, std::min<int64_t>({512 / grid, (most + LEAST - 1) / LEAST, 64}));
+    torch::Tensor part;
+    if (slices > 1) {
+      const int64_t n = slices * T * H;
+      part = torch::empty({n * (D + 2)}, q.options().dtype(at::kFloat));
+      a.o_part = part.data_ptr<float>();
+      a.ml_part = a.o_part + n * D;
+    }
+    hipLaunchKernelGGL((chunk_attn_kernel<DIM, NW>), dim3(grid, slices), dim3(NW * 64),
+                       4 * TILE * DIM * 2, stream, a);
+    HIP_CHECK_LAST();
+    if (slices > 1) {
       hipLaunchKernelGGL(chunk_join_kernel<DIM>, dim3(CDIV(T * H * (DIM / 8), 256)), dim3(256), 0,
                          stream, a, slices);
       HIP_CHECK_LAST();
     }
   };
-  // 256 rows a workgroup read K and V half as often, where sequences have so many and there
-  // are enough of them, and where their fuller start is made up for: 2 x 4096 behind 8192,
-  // 64/8 heads 2793 us with 128 rows, 2611 so; 2048 behind 14336, 28/4 505 and 482; 16 x
-  // 20..120 behind 1040 45.3 and 43.0; but 10 x 200..350 behind none 27.0 and 30.9, single
-  // tokens among two chunks 97 and 133.
-  const bool wide = T * (H / KV) >= 256 * B && most >= 1024 && grid_of(256) >= 160;
-  constexpr std::integral_constant<int, 4> four{};
-  if (D == 128 && wide) go(std::integral_constant<int, 128>{}, std::integral_constant<int, 8>{});
-  else if (D == 128) go(std::integral_constant<int, 128>{}, four);
-  else go(std::integral_constant<int, 64>{}, four);
+  // By rows of a sequence, keys a row sees on average (if sequences are alike and their
+  // tables as wide as they need) and workgroups. us, light and deep kernel, 128 rows and
+  // 256 a workgroup: 2 x 4096 behind 8192, 64/8 heads 2975 and 2711; 2048 behind 14336, 28/4
+  // 558 and 503; 8192 behind none, 28/4 538 and 514; 16 x 20..120 behind 1040, 28/4 46.4 and
+  // 44.2; but 4 x 1200 behind none 66.8 and 76.3, 10 x 200..350 22.1 and 30.7, single
+  // tokens among two chunks 99.7 and 138.
+  if (D == 128 && T * (H / KV) >= 256 * B && most - T / (2 * B) >= 1024 && grid_of(256) >= 160)
+    deep();
+  else if (D == 128)
+    light(std::integral_constant<int, 128>{});
+  else
+    light(std::integral_constant<int, 64>{});
   return out;
 }
