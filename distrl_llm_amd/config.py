@@ -86,10 +86,15 @@ class EngineConfig:
     # Automatic cross-request prefix caching (vLLM APC analogue): full
     # prompt blocks are kept in the pool keyed by their token prefix and
     # reused by later requests sharing the prefix (classic win: a long
-    # system prompt + short user tails). Cache-hit tails prefill through
-    # the decode step (existing kernels only); LRU-evicted under pool
+    # system prompt + short user tails). Cache-hit tails prefill in one flat
+    # batch that attends to the cached pages; LRU-evicted under pool
     # pressure. Off by default: RL rollouts use unique prompts.
     enable_prefix_caching: bool = False
+    # When >0, most prompt tokens a prefill step of a dense model carries:
+    # longer prompts run in chunks, each attending to the pages of those
+    # before it, which bounds the activations a prompt phase holds. 0: all
+    # tokens of a prefill batch at once.
+    prefill_chunk_tokens: int = 0
     # Layer-list (hybrid) models: number of per-sequence state slots
     # (convolution tails, recurrent state); it bounds the live sequences.
     # 0 = min(max_num_seqs, 256).

@@ -343,6 +343,9 @@ def main():
     ap.add_argument("--enable-prefix-caching", action="store_true",
                     help="reuse KV blocks of shared prompt prefixes "
                          "across requests (vLLM APC analogue)")
+    ap.add_argument("--prefill-chunk-tokens", type=int, default=0,
+                    help="most prompt tokens of one prefill step; longer "
+                         "prompts run in chunks (0: no bound)")
     args = ap.parse_args()
 
     device = torch.device("cuda:0" if torch.cuda.is_available() else "cpu")
@@ -351,9 +354,10 @@ def main():
     if hybrid_design_of(args.model) is not None:
         # a layer-list design: config.json names it, the registry builds
         # its model and engine (same generate() contract)
-        if args.adapter or args.enable_prefix_caching:
-            raise SystemExit("--adapter / --enable-prefix-caching apply to "
-                             "the dense model families only")
+        if args.adapter or args.enable_prefix_caching or args.prefill_chunk_tokens:
+            raise SystemExit("--adapter / --enable-prefix-caching / "
+                             "--prefill-chunk-tokens apply to the dense model "
+                             "families only")
         model, engine = load_model_and_engine(
             args.model, EngineConfig(
                 max_seq_length=args.max_seq_length,
@@ -383,7 +387,8 @@ def main():
     engine = Engine(model, EngineConfig(
         max_seq_length=args.max_seq_length,
         gpu_memory_utilization=args.gpu_memory_utilization,
-        enable_prefix_caching=args.enable_prefix_caching),
+        enable_prefix_caching=args.enable_prefix_caching,
+        prefill_chunk_tokens=args.prefill_chunk_tokens),
         device=device, seed=args.seed)
 
     import uvicorn
