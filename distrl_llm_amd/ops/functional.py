@@ -177,8 +177,8 @@ def paged_attention_chunk(q, key_cache, value_cache, block_tables, cu,
 
     bfloat16 and head_dim 64 or 128 on the GPU. No gradient: the cache serves
     generation."""
-    if torch.is_grad_enabled() and any(
-            t.requires_grad for t in (q, key_cache, value_cache)):
+    if torch.is_grad_enabled() and (q.requires_grad or key_cache.requires_grad
+                                    or value_cache.requires_grad):
         raise RuntimeError("paged_attention_chunk has no gradient: call it "
                            "under torch.no_grad()")
     if not 0.0 < scale < 1e30 or longest < 0:
@@ -186,10 +186,12 @@ def paged_attention_chunk(q, key_cache, value_cache, block_tables, cu,
     if q.is_cuda:
         ext = _require_ext("paged_attention_chunk")
         if ext is not None:
+            if not (block_tables.dtype == cu.dtype == context_lens.dtype == torch.int32):
+                block_tables, cu, context_lens = (
+                    t.to(torch.int32) for t in (block_tables, cu, context_lens))
             return ext.paged_attention_chunk(
-                q, key_cache, value_cache, block_tables.to(torch.int32).contiguous(),
-                cu.to(torch.int32).contiguous(),
-                context_lens.to(torch.int32).contiguous(), float(scale), int(longest))
+                q, key_cache, value_cache, block_tables.contiguous(), cu.contiguous(),
+                context_lens.contiguous(), scale, longest)
     return R.paged_attention_chunk(q, key_cache, value_cache, block_tables, cu,
                                    context_lens, scale)
 
@@ -219,6 +221,11 @@ def chunk_slots(block_tables, context_lens, new_lens, pages, block_size: int,
     tokens past a table's end and those whose page is missing or negative get
     cache row -1, which the writers of the cache skip. A request without new
     tokens has the row before it as its last one."""
+    if block_tables.is_cuda:
+        ext = _require_ext("chunk_slots")
+        if ext is not None:
+            return ChunkSlots(*ext.chunk_slots(block_tables, context_lens, new_lens,
+                                               pages, block_size, rows, held))
     for t in (block_tables, context_lens, new_lens, pages, held):
         if t is not None and (t.dtype != torch.int32 or not t.is_contiguous()
                               or t.device != block_tables.device):
@@ -228,11 +235,6 @@ def chunk_slots(block_tables, context_lens, new_lens, pages, block_size: int,
             for t in (context_lens, new_lens, held)):
         raise ValueError("chunk_slots: block_tables (requests, pages), a length "
                          "for each request, a block size and rows")
-    if block_tables.is_cuda:
-        ext = _require_ext("chunk_slots")
-        if ext is not None:
-            return ChunkSlots(*ext.chunk_slots(block_tables, context_lens, new_lens,
-                                               pages, int(block_size), int(rows), held))
     return ChunkSlots(*R.chunk_slots(block_tables, context_lens, new_lens, pages,
                                      block_size, rows, held))
 
