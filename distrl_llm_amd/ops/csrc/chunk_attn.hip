@@ -9,18 +9,18 @@
 // A workgroup owns a kv head and a block of rows that are (token, query head of the
 // group) pairs, tokens outermost: K and V are read once for all heads of the group, and a
 // block ends few tokens behind its first, so that little of the diagonal is computed in
-// vain. Products and softmax are those of the learner's attention (attention_tiles.h). Two
-// kernels share them: a light one and one for many rows over long contexts.
+// vain. Products and softmax are those of the learner's attention (attention_tiles.h). Three
+// kernels share them: a light one, one for many rows over long contexts and one for few.
 //
-// 2 x 4096 behind 8192, 64/8 heads of 128 2711 us = 1014 TFLOP/s (a product of 8192^3
+// 2 x 4096 behind 8192, 64/8 heads of 128 2690 us = 1022 TFLOP/s (a product of 8192^3
 // 1296), where the matrix cores are busy half of the time: a SIMD's two waves have 512
 // cycles of products and 620 of vector work each a block of 32 keys, and little of one's
 // hides behind the other's. Tried there: 128 rows a workgroup 2796, the light kernel 2975,
 // 64 rows a wave (one wave a SIMD) 3755, weights used a turn later (spills) 2959,
 // priorities of waves even. 6 single tokens behind 20 to 32 thousand, 40/8 heads 126 us =
-// 4.5 TB/s, K and V read once. 16 x 20..120 behind 1040, 28/4 44 us, 10 x 200..350 behind
+// 4.5 TB/s, K and V read once. 16 x 20..120 behind 1040, 28/4 43 us, 10 x 200..350 behind
 // none 22: a workgroup's start (lengths, pages, rows, one behind the other) and 9 to 35
-// blocks of 0.7 us.
+// blocks of 0.7 us. 5 tokens behind 1040, 14/2 of 64 10.6: two launches of such chains.
 #include <torch/extension.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -116,7 +116,8 @@ struct Work {
   bool live;
 };
 
-// Whether there is any work; if not, rows of no sequence have been cleared.
+// Whether there is any work; if not, rows of no sequence have been cleared. NW waves own 32
+// rows each, or one block of them is every wave's.
 template <int D, int NW>
 DEV_INLINE bool find_work(const Chunk& a, Work& w) {
   constexpr int ROWS = NW * WROWS;
@@ -134,7 +135,7 @@ DEV_INLINE bool find_work(const Chunk& a, Work& w) {
   const int before = w.q.ctx - (w.q.end - w.q.first);
   const int reach = (int)min((int64_t)a.width * a.block, (int64_t)1 << 30);
   auto keys_of = [&](int r) { return max(0, min(before + a.by_group.of(r) + 1, reach)); };
-  const int r0 = w.block0 + wave_id() * WROWS, row = r0 + (threadIdx.x & 31);
+  const int r0 = w.block0 + (NW == 1 ? 0 : wave_id() * WROWS), row = r0 + (threadIdx.x & 31);
   const int r = min(row, w.rows - 1), of = a.by_group.of(r);
   w.live = row < w.rows;
   w.t = w.q.first + of;
@@ -248,10 +249,10 @@ DEV_INLINE void finish(const Chunk& a, const Work& w, float m, float lsum, f32x1
 
 // Rows of K and V of a tile: fetched into registers, then stored to LDS. Rows
 // past the end and pages that are none read as zeros.
-template <int D, int NT>
+template <int D, int KEYS, int NT>
 struct Staged {
-  static constexpr int UN = D / 8, STEP = NT / UN, PER = TILE / STEP;
-  static_assert(TILE % STEP == 0, "tile does not divide");
+  static constexpr int UN = D / 8, STEP = NT / UN, PER = KEYS / STEP;
+  static_assert(KEYS % STEP == 0, "tile does not divide");
   u32x4 k[PER], v[PER];
   int page[PER];                // of the rows that are fetched next
   int there;                    // a bit a row: k and v hold it
@@ -313,7 +314,7 @@ void chunk_attn_kernel(Chunk a) {
   if (w.begin < w.end) {
     const int* table = a.tables + (int64_t)w.q.b * a.width;
     const int most = __builtin_amdgcn_readlane(w.mine, 31);       // of the wave's rows
-    Staged<D, NW * 64> tile;
+    Staged<D, TILE, NW * 64> tile;
     tile.look(a, table, w.begin, w.end);
     tile.fetch(a, kv, w.begin, w.end);
     tile.look(a, table, w.begin + TILE, w.end);
@@ -360,6 +361,107 @@ void chunk_attn_kernel(Chunk a) {
     }
   }
   finish<D>(a, w, m, lsum, acc);
+}
+
+// Few rows of a sequence, as single tokens: a workgroup's four waves have the same 32 rows
+// and 32 keys of a tile of 128 each, with a softmax of their own, joined at the end. (One
+// wave for all keys of a tile is a chain four times as long, beside three that wait.)
+template <int D>
+__global__ __launch_bounds__(256, 2)
+void chunk_few_kernel(Chunk a) {
+  constexpr int NW = 4, KEYS = NW * 32, TB = KEYS * D * 2, LD = D + 4;
+  Work w;
+  if (!find_work<D, 1>(a, w)) return;
+  const int kv = blockIdx.x % a.KV, wave = wave_id();
+  extern __shared__ __attribute__((aligned(256))) char smem[];
+  const Frags<D> fr;
+  bf16v8 qf[D / 16];
+  load_queries<D>(a, w, qf);
+  float m = -1e30f, lsum = 0.f;
+  f32x16 acc[D / 32];
+  #pragma unroll
+  for (int dt = 0; dt < D / 32; ++dt) acc[dt] = zero16();
+
+  if (w.begin < w.end) {
+    const int* table = a.tables + (int64_t)w.q.b * a.width;
+    Staged<D, KEYS, NW * 64> tile;
+    tile.look(a, table, w.begin, w.end);
+    tile.fetch(a, kv, w.begin, w.end);
+    tile.look(a, table, w.begin + KEYS, w.end);
+    for (int t0 = w.begin; t0 < w.end; t0 += KEYS) {
+      tile.store(smem, smem + TB);
+      __syncthreads();
+      if (t0 + KEYS < w.end) {
+        tile.fetch(a, kv, t0 + KEYS, w.end);
+        tile.look(a, table, t0 + 2 * KEYS, w.end);
+      }
+      const int k0 = t0 + wave * 32;
+      if (k0 < w.end) {                                 // wave-uniform
+        f32x16 st[1] = {zero16()};
+        #pragma unroll
+        for (int ks = 0; ks < D / 16; ++ks) st[0] = mfma(fr.row(smem, wave, ks), qf[ks], st[0]);
+        if (k0 + 32 > min(w.least, w.end)) hide(st[0], w, k0);
+        bf16v8 p[1][2];
+        float sum;
+        const float fall = weigh(st, p, m, sum, w.mine <= FEW, a.scale_log2);
+        if (__any(fall < 0.f)) rescale<D>(fall, lsum, acc);
+        lsum += sum;
+        #pragma unroll
+        for (int k2 = 0; k2 < 2; ++k2)
+          #pragma unroll
+          for (int dt = 0; dt < D / 32; ++dt)
+            acc[dt] = mfma(fr.col(smem + TB, wave * 32 + k2 * 16, dt), p[0][k2], acc[dt]);
+      }
+      __syncthreads();
+    }
+  }
+
+  float* parts = reinterpret_cast<float*>(smem);        // (waves, 32, LD), then (waves, 32, 2)
+  float* ml = parts + NW * WROWS * LD;
+  const int l = threadIdx.x & 63;
+  lsum = halves_sum(lsum);
+  store_rows_f32<D>(acc, parts + (wave * WROWS + (l & 31)) * LD, true);
+  if (l < 32) {
+    const bool seen = min(w.mine, w.end) > w.begin + wave * 32;
+    ml[(wave * WROWS + l) * 2] = seen ? m : -1e30f;
+    ml[(wave * WROWS + l) * 2 + 1] = seen ? lsum : 0.f;
+  }
+  __syncthreads();
+  const int row = threadIdx.x / 8, r = w.block0 + row, of = a.by_group.of(r);
+  if (r >= w.rows) return;
+  float top = -1e30f, total = 0.f, f[NW];
+  #pragma unroll
+  for (int i = 0; i < NW; ++i) top = fmaxf(top, ml[(i * WROWS + row) * 2]);
+  #pragma unroll
+  for (int i = 0; i < NW; ++i) {
+    const float sum = ml[(i * WROWS + row) * 2 + 1];
+    f[i] = sum > 0.f ? __builtin_amdgcn_exp2f(ml[(i * WROWS + row) * 2] - top) : 0.f;
+    total += f[i] * sum;
+  }
+  const int64_t at = (int64_t)(w.q.first + of) * a.H + kv * a.by_group.n + r - of * a.by_group.n;
+  const int64_t part = blockIdx.y * (int64_t)a.T * a.H + at;
+  #pragma unroll
+  for (int d0 = 0; d0 < D / 8; d0 += 4) {
+    const int d = threadIdx.x % 8 * 4 + d0 * 8;
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+    #pragma unroll
+    for (int i = 0; i < NW; ++i)
+      if (f[i] > 0.f)           // else what is there is no number
+        o += f[i] * *reinterpret_cast<const f32x4*>(parts + (i * WROWS + row) * LD + d);
+    if (gridDim.y > 1) {
+      *reinterpret_cast<f32x4*>(a.o_part + part * D + d) = o;
+      continue;
+    }
+    const float inv = total > 0.f ? 1.f / total : 0.f;
+    bf16v4 y;
+    #pragma unroll
+    for (int j = 0; j < 4; ++j) y[j] = (__bf16)(o[j] * inv);
+    *reinterpret_cast<bf16v4*>(a.out + at * D + d) = y;
+  }
+  if (gridDim.y > 1 && threadIdx.x % 8 == 0) {
+    a.ml_part[part * 2] = top;
+    a.ml_part[part * 2 + 1] = total;
+  }
 }
 
 // Addresses of a block's fragments, in registers: which block it is goes into the
@@ -721,9 +823,10 @@ torch::Tensor paged_attention_chunk(torch::Tensor q, torch::Tensor kcache, torch
                        dim3(NW * 64), lds, stream, a);
     HIP_CHECK_LAST();
   };
-  auto light = [&](auto d_) {
-    constexpr int DIM = decltype(d_)::value, NW = 4;
-    const int64_t grid = check(grid_of(NW * WROWS));
+  auto sliced = [&](auto d_, auto few_) {
+    constexpr int DIM = decltype(d_)::value;
+    constexpr bool FEWS = decltype(few_)::value;
+    const int64_t grid = check(grid_of(FEWS ? WROWS : 4 * WROWS));
     // Slices where the workgroups leave CUs idle (two of four waves a CU), of 256 keys at
     // least and from three of them on: the join is a launch of 4 us. 5 tokens behind 1040,
     // 14/2 heads of 64 12.2 us, one slice 18.
@@ -736,8 +839,18 @@ torch::Tensor paged_attention_chunk(torch::Tensor q, torch::Tensor kcache, torch
       a.o_part = part.data_ptr<float>();
       a.ml_part = a.o_part + n * D;
     }
-    hipLaunchKernelGGL((chunk_attn_kernel<DIM, NW>), dim3(grid, slices), dim3(NW * 64),
-                       4 * TILE * DIM * 2, stream, a);
+    const dim3 launch(grid, slices);
+    if constexpr (FEWS) {
+      constexpr int lds = 4 * WROWS * (DIM + 6) * 4;
+      static_assert(lds >= 4 * 4 * WROWS * DIM, "tile and join share LDS");
+      static const hipError_t raised = hipFuncSetAttribute(
+          reinterpret_cast<const void*>(chunk_few_kernel<DIM>),
+          hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+      TORCH_CHECK(raised == hipSuccess, "paged_attention_chunk: LDS");
+      hipLaunchKernelGGL(chunk_few_kernel<DIM>, launch, dim3(256), lds, stream, a);
+    } else {
+      hipLaunchKernelGGL((chunk_attn_kernel<DIM, 4>), launch, dim3(256), 4 * TILE * DIM * 2, stream, a);
+    }
     HIP_CHECK_LAST();
     if (slices > 1) {
       hipLaunchKernelGGL(chunk_join_kernel<DIM>, dim3(CDIV(T * H * (DIM / 8), 256)), dim3(256), 0,
@@ -751,11 +864,20 @@ torch::Tensor paged_attention_chunk(torch::Tensor q, torch::Tensor kcache, torch
   // 558 and 503; 8192 behind none, 28/4 538 and 514; 16 x 20..120 behind 1040, 28/4 46.4 and
   // 44.2; but 4 x 1200 behind none 66.8 and 76.3, 10 x 200..350 22.1 and 30.7, single
   // tokens among two chunks 99.7 and 138.
+  // Up to 64 rows a sequence, where a step waits for chains and not for memory. us, light
+  // kernel and few rows: a token behind 1000, 14/2 heads of 64 10.9 and 9.7, 40/8 of 128
+  // 14.0 and 12.5; 64 x 1 behind 500, 14/2 11.6 and 7.7; but 8 x 1 behind 2000, 28/4 of 128
+  // 18.1 and 20.1, 64 x 1 behind 3000 93.7 and 107 (40/8 207 and 184).
+  const bool few = longest * (H / KV) <= 64 && (D == 64 || B == 1);
+  auto by_rows = [&](auto d_) {
+    if (few) sliced(d_, std::true_type{});
+    else sliced(d_, std::false_type{});
+  };
   if (D == 128 && T * (H / KV) >= 256 * B && most - T / (2 * B) >= 1024 && grid_of(256) >= 160)
     deep();
   else if (D == 128)
-    light(std::integral_constant<int, 128>{});
+    by_rows(std::integral_constant<int, 128>{});
   else
-    light(std::integral_constant<int, 64>{});
+    by_rows(std::integral_constant<int, 64>{});
   return out;
 }

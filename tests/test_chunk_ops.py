@@ -79,8 +79,8 @@ def exact(q, key_cache, value_cache, block_tables, cu, context_lens, scale, long
     return out[0], out[1]
 
 
-def check(case, got):
-    want, size = exact(**case)
+def check(case, got, oracle=exact):
+    want, size = oracle(**case)
     bound = want.abs() * 2.0 ** -8 + size * (2.0 ** -8 + 2.0 ** -12) + 1e-30
     if case["q"].dtype == torch.float32:
         bound = size * 2.0 ** -14 + 1e-30
@@ -124,6 +124,118 @@ def test_attention_long(new, cached, heads, kv, dim):
     """Contexts that are cut into slices and joined."""
     case = make(heads, kv, dim, 16, new, cached, seed=heads, device="cuda")
     check(case, OF.paged_attention_chunk(**case))
+
+
+def exact_fast(q, key_cache, value_cache, block_tables, cu, context_lens, scale, longest):
+    """exact() for many rows: all rows of a sequence and kv head at once."""
+    q, tables = q.cpu().double(), block_tables.cpu().long()
+    cu, lens = cu.tolist(), context_lens.tolist()
+    pages, block, kv, dim = key_cache.shape
+    group = q.shape[1] // kv
+    out = torch.zeros(2, *q.shape, dtype=torch.float64)
+    for b, (first, end) in enumerate(zip(cu, cu[1:])):
+        at = torch.arange(lens[b])
+        page = tables[b][at // block]
+        there = ((page >= 0) & (page < pages)).view(-1, 1, 1)
+        line = page.clamp(0, pages - 1) * block + at % block
+        k, v = (torch.where(there, c.cpu().view(-1, kv, dim)[line].double(), 0.0)
+                for c in (key_cache, value_cache))
+        later = at[None, :] > (lens[b] - (end - first) + torch.arange(end - first))[:, None]
+        for h in range(q.shape[1]):
+            w = torch.softmax((q[first:end, h] @ k[:, h // group].T * scale)
+                              .masked_fill(later, -math.inf), 1)
+            out[0, first:end, h] = w @ v[:, h // group]
+            out[1, first:end, h] = w @ v[:, h // group].abs()
+    return out[0], out[1]
+
+
+DEEP = [  # the kernel for many rows over long contexts: at least 160 workgroups of 256
+    dict(heads=64, kv=8, block=16, new=[640], cached=[1700]),
+    dict(heads=64, kv=8, block=5, new=[500, 33, 1, 700], cached=[1500, 2300, 1999, 1100]),
+    dict(heads=64, kv=8, block=64, new=[700, 300], cached=[1037, 1987]),
+    dict(heads=32, kv=32, block=16, new=[1100, 400], cached=[1024, 1777]),
+    dict(heads=20, kv=20, block=16, new=[2300], cached=[0], spare=100),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", DEEP)
+def test_attention_deep(case):
+    case = make(dim=128, device="cuda", seed=len(case["new"]), **case)
+    check(case, OF.paged_attention_chunk(**case), exact_fast)
+
+
+@pytest.mark.gpu
+def test_attention_deep_with_pages_outside():
+    """Rows of such pages read as zeros, whatever lies there, in every block."""
+    case = make(64, 8, 128, 16, [600, 100], [1500, 1300], device="cuda")
+    tables = case["block_tables"]
+    tables[0, 3], tables[0, 70], tables[1, 64], tables[0, 131] = -1, 1 << 30, -(1 << 31), 10 ** 6
+    check(case, OF.paged_attention_chunk(**case), exact_fast)
+    few = {**case, "cu": torch.tensor([100, 600, 700], dtype=torch.int32, device="cuda")}
+    got = OF.paged_attention_chunk(**few)
+    assert not bool(got[:100].any())
+    check(few, got, exact_fast)
+
+
+@pytest.mark.gpu
+def test_attention_deep_in_a_cache_past_32_bits():
+    case = make(64, 8, 128, 16, [640], [1700], device="cuda", stale=0.5)
+    small = case["key_cache"].shape[0]
+    pages = 2 ** 32 // (16 * 8 * 128 * 2) + small
+    far = {n: torch.empty(pages, 16, 8, 128, dtype=torch.bfloat16, device="cuda")
+           for n in ("key_cache", "value_cache")}
+    for n, c in far.items():
+        c[pages - small:] = case[n]
+    tables = case["block_tables"]
+    moved = torch.where(tables < small, tables + (pages - small), tables)
+    got = OF.paged_attention_chunk(**{**case, **far, "block_tables": moved})
+    assert torch.equal(got, OF.paged_attention_chunk(**case))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("heads,kv,dim", [(14, 2, 64), (64, 8, 128), (28, 4, 128)])
+def test_attention_does_not_hang_on_the_batch(heads, kv, dim):
+    """A row's result alone, in a batch and in chunks of its sequence: the same softmax in
+    other tiles and slices, so rounded alike but for the order of fp32 sums."""
+    case = make(heads, kv, dim, 16, [700, 5, 90], [900, 1300, 40], device="cuda")
+    want = OF.paged_attention_chunk(**case).float()
+    for b, first, end in ((0, 0, 700), (1, 700, 705), (2, 705, 795)):
+        for rows in (1, 5, 64, 1000):
+            for at in range(max(first, end - 200), end, 200 if rows > 64 else 67):
+                stop = min(at + rows, end)
+                lens = case["context_lens"][b:b + 1] - (end - stop)
+                one = {**case, "q": case["q"][at:stop], "context_lens": lens,
+                       "block_tables": case["block_tables"][b:b + 1], "longest": stop - at,
+                       "cu": torch.tensor([0, stop - at], dtype=torch.int32, device="cuda")}
+                got = OF.paged_attention_chunk(**one).float()
+                share = (got != want[at:stop]).float().mean()
+                assert float(share) < 0.02, (b, rows, at)
+
+
+@pytest.mark.gpu
+def test_attention_of_one_key_is_its_value():
+    case = make(8, 2, 64, 16, [1, 1, 1], [0, 0, 0], device="cuda")
+    got = OF.paged_attention_chunk(**case).unflatten(1, (2, 4))
+    page = case["block_tables"][:, 0].long()
+    assert torch.equal(got, case["value_cache"][page, 0].unsqueeze(2).expand_as(got))
+
+
+@pytest.mark.gpu
+def test_two_streams_at_once():
+    """Calls that overlap have workspaces of their own."""
+    cases = [make(28, 4, 128, 16, [3], [6000 + 500 * i], seed=i, device="cuda") for i in range(4)]
+    want = [OF.paged_attention_chunk(**c) for c in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    got = [[] for _ in cases]
+    for _ in range(8):
+        for c, s, out in zip(cases, streams, got):
+            with torch.cuda.stream(s):
+                out.append(OF.paged_attention_chunk(**c))
+    torch.cuda.synchronize()
+    for w, outs in zip(want, got):
+        assert all(torch.equal(w, o) for o in outs)
 
 
 @pytest.mark.gpu
