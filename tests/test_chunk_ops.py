@@ -326,6 +326,27 @@ def test_captured_step(new, cached):
         assert torch.equal(got, want), turn
 
 
+def check_empty(device, dtype, dim):
+    case = make(8, 2, dim, 16, [4, 5], [20, 0], device=device, dtype=dtype, stale=0.5)
+    none = torch.zeros(0, dtype=torch.int32, device=device)
+    got = OF.paged_attention_chunk(**{**case, "q": case["q"][:0], "cu": case["cu"] * 0})
+    assert got.shape == (0, 8, dim)
+    got = OF.paged_attention_chunk(**{**case, "block_tables": case["block_tables"][:0],
+                                      "cu": case["cu"][:1], "context_lens": none})
+    assert got.shape == case["q"].shape and not bool(got.any())
+    got = OF.paged_attention_chunk(**{**case, "cu": case["cu"] * 0})
+    assert not bool(got.any())
+
+
+def test_empty_batches_cpu():
+    check_empty("cpu", torch.float32, 16)
+
+
+@pytest.mark.gpu
+def test_empty_batches():
+    check_empty("cuda", torch.bfloat16, 64)
+
+
 def misuse(case):
     yield "no key before a row", {"context_lens": torch.tensor([2, 0], dtype=torch.int32)}
     yield "table ends early", {"block_tables": case["block_tables"][:, :1].contiguous()}
@@ -414,6 +435,8 @@ def slots_cases():
     yield dict(ctx=[10, 0], new=[30, 20], block=8, free=3)         # too few pages
     yield dict(ctx=[10, 0], new=[30, 20], block=8, width=3)        # tables too narrow
     yield dict(ctx=[i % 50 for i in range(300)], new=[(i * 7) % 23 for i in range(300)], block=16)
+    yield dict(ctx=[], new=[], block=16, rows=3)                   # no request
+    yield dict(ctx=[3, 4], new=[2, 0], block=16, rows=0)           # no row
     yield dict(ctx=[0] * 257, new=[1] * 257, block=16)
     yield dict(ctx=[0] * 3, new=[4000, 1, 2500], block=16)
 
