@@ -90,11 +90,6 @@ class EngineConfig:
     # batch that attends to the cached pages; LRU-evicted under pool
     # pressure. Off by default: RL rollouts use unique prompts.
     enable_prefix_caching: bool = False
-    # When >0, most prompt tokens a prefill step of a dense model carries:
-    # longer prompts run in chunks, each attending to the pages of those
-    # before it, which bounds the activations a prompt phase holds. 0: all
-    # tokens of a prefill batch at once.
-    prefill_chunk_tokens: int = 0
     # Layer-list (hybrid) models: number of per-sequence state slots
     # (convolution tails, recurrent state); it bounds the live sequences.
     # 0 = min(max_num_seqs, 256).
@@ -102,3 +97,8 @@ class EngineConfig:
     # Hybrid models: most tokens one step carries (decode tokens first,
     # prompt portions fill the rest).
     step_token_budget: int = 8192
+    # When >0, most prompt tokens a prefill step of a dense model carries:
+    # longer prompts run in chunks, each attending to the pages of those
+    # before it, which bounds the activations a prompt phase holds. 0: all
+    # tokens of a prefill batch at once.
+    prefill_chunk_tokens: int = 0

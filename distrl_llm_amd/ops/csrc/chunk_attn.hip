@@ -527,7 +527,8 @@ struct Paged {
   uint32_t step;                // bytes from cache row to row
 
   DEV_INLINE int row(int n) const { return (wave_id() * PER + n) * (64 / UN) + (threadIdx.x & 63) / UN; }
-  DEV_INLINE Paged(const Chunk& a, uint32_t lds, int kv) : lds(lds), value(reinterpret_cast<uint64_t>(a.value) - reinterpret_cast<uint64_t>(a.key)),
+  DEV_INLINE Paged(const Chunk& a, uint32_t lds, int kv)
+      : lds(lds), value(reinterpret_cast<uint64_t>(a.value) - reinterpret_cast<uint64_t>(a.key)),
         step(a.KV * D * 2) {
     #pragma unroll
     for (int n = 0; n < PER; ++n) {
@@ -587,10 +588,10 @@ struct Paged {
   }
 };
 
-// Many rows and long contexts: keys come in blocks of 32 through rings of four in LDS. A turn of the
-// loop makes the weights of block i beside the products with the keys of block i + 1,
-// which wait in registers, then adds the values of block i while the keys of block i + 2
-// are read; the keys of block i + 5 and the values of i + 3 set out meanwhile.
+// Many rows and long contexts: keys come in blocks of 32 through rings of four in LDS. A
+// turn of the loop makes the weights of block i beside the products with the keys of block
+// i + 1, which wait in registers, then adds the values of block i while the keys of block
+// i + 2 are read; the keys of block i + 5 and the values of i + 3 set out meanwhile.
 template <int D, int NW>
 __global__ __launch_bounds__(NW * 64, 2)
 void chunk_deep_kernel(Chunk a) {
@@ -827,11 +828,13 @@ torch::Tensor paged_attention_chunk(torch::Tensor q, torch::Tensor kcache, torch
     constexpr int DIM = decltype(d_)::value;
     constexpr bool FEWS = decltype(few_)::value;
     const int64_t grid = check(grid_of(FEWS ? WROWS : 4 * WROWS));
-    // Slices where the workgroups leave CUs idle (two of four waves a CU), of 256 keys at
-    // least and from three of them on: the join is a launch of 4 us. 5 tokens behind 1040,
-    // 14/2 heads of 64 12.2 us, one slice 18.
+    // Slices where the workgroups leave CUs idle (a CU holds two of four waves, with heads
+    // of 64 four), of 256 keys at least and from three of them on: the join is a launch of 4
+    // us. 5 tokens behind 1040, 14/2 heads of 64 12.2 us, one slice 18. Half and twice as
+    // many: 36 x 43..68 behind up to 8435, 8/2 of 64 92.5 and 57.4, 2 x 36..826 behind 6000,
+    // 32/8 of 128 40.0 and 44.6.
     const int slices = most < 3 * LEAST ? 1 : (int)std::max<int64_t>(
-        1, std::min<int64_t>({512 / grid, (most + LEAST - 1) / LEAST, 64}));
+        1, std::min<int64_t>({(DIM == 64 ? 1024 : 512) / grid, (most + LEAST - 1) / LEAST, 64}));
     torch::Tensor part;
     if (slices > 1) {
       const int64_t n = slices * T * H;
