@@ -16,7 +16,7 @@
 // 1296), where the matrix cores are busy half of the time: a SIMD's two waves have 512
 // cycles of products and 620 of vector work each a block of 32 keys, and little of one's
 // hides behind the other's. Tried there: 128 rows a workgroup 2796, the light kernel 2975,
-// 64 rows a wave (one wave a SIMD) 3755, weights used a turn later (spills) 2959,
+// 64 rows a wave (one wave a SIMD) 3755, twelve waves of 32 (three a SIMD) 2856 for 2767,
 // priorities of waves even. 6 single tokens behind 20 to 32 thousand, 40/8 heads 126 us =
 // 4.5 TB/s, K and V read once. 16 x 20..120 behind 1040, 28/4 43 us, 10 x 200..350 behind
 // none 22: a workgroup's start (lengths, pages, rows, one behind the other) and 9 to 35
