@@ -12,15 +12,16 @@
 // vain. Products and softmax are those of the learner's attention (attention_tiles.h). Three
 // kernels share them: a light one, one for many rows over long contexts and one for few.
 //
-// 2 x 4096 behind 8192, 64/8 heads of 128 2690 us = 1022 TFLOP/s (a product of 8192^3
-// 1296), where the matrix cores are busy half of the time: a SIMD's two waves have 512
-// cycles of products and 620 of vector work each a block of 32 keys, and little of one's
-// hides behind the other's. Tried there: 128 rows a workgroup 2796, the light kernel 2975,
-// 64 rows a wave (one wave a SIMD) 3755, twelve waves of 32 (three a SIMD) 2856 for 2767,
-// priorities of waves even. 6 single tokens behind 20 to 32 thousand, 40/8 heads 126 us =
-// 4.5 TB/s, K and V read once. 16 x 20..120 behind 1040, 28/4 43 us, 10 x 200..350 behind
-// none 22: a workgroup's start (lengths, pages, rows, one behind the other) and 9 to 35
-// blocks of 0.7 us. 5 tokens behind 1040, 14/2 of 64 10.6: two launches of such chains.
+// Weights go into the second product as two bf16 terms, 17 bits, as those of single tokens
+// do (paged_attn.hip); the result's error against 64 bits is then that of its own rounding
+// (0.00166, with one term 0.0023). It costs half as much matrix work again: 2 x 4096 behind
+// 8192, 64/8 heads of 128 3480 us for 2670, 1180 TFLOP/s with the second terms (a product
+// of 8192^3 1296). Tried there, with one term: 128 rows a workgroup 2796, the light kernel
+// 2975, 64 rows a wave (one wave a SIMD) 3755, twelve waves of 32 (three a SIMD) 2856 for
+// 2767, priorities of waves even. 6 single tokens behind 20 to 32 thousand, 40/8 heads 128
+// us = 4.5 TB/s, K and V read once. 16 x 20..120 behind 1040, 28/4 50 us, 10 x 200..350
+// behind none 24: a workgroup's start (lengths, pages, rows, one behind the other) and 6 to
+// 35 blocks or tiles. 5 tokens behind 1040, 14/2 of 64 11: two launches of such chains.
 #include <torch/extension.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -32,7 +33,6 @@ constexpr int BLOCK = 32, RING = 4;     // keys of a block of the deep kernel, b
 constexpr int AHEAD = 1024;             // keys whose cache rows are looked up at once
 constexpr int TILE = 64;        // keys of a tile
 constexpr int LEAST = 256;      // of a slice, at least
-constexpr int FEW = 16;
 
 // x / n for 0 <= x < 2^30 as a product: ceil(2^(31 + shift) / n), shift = ceil(log2(n)), is
 // too large by less than 1 and x times that less than 2^(31 + shift), so the result is exact.
@@ -164,24 +164,31 @@ DEV_INLINE void hide(f32x16& st, const Work& w, int k0) {
     if (seen <= acc_row(j, 0)) st[j] = -1e30f;
 }
 
-// x + the sum of eight
-DEV_INLINE float pair_sum(const bf16v8& v, float x) {
-  const bf16v2 ones = {(__bf16)1.f, (__bf16)1.f};
+// The second term of weights 8 k .. 8 k + 7, whose first is hi = pack8(p, k): p = hi + lo,
+// off by 2^-16 of p at most. (Made and used beside the products with hi: with those of both
+// terms behind it all 2 x 4096 behind 8192 take 3816 us for 3480.)
+DEV_INLINE bf16v8 rest8(const f32x16& p, const bf16v8& hi, int k) {
+  f32x16 rest;
   #pragma unroll
-  for (int j = 0; j < 8; j += 2) x = __builtin_amdgcn_fdot2_f32_bf16(bf16v2{v[j], v[j + 1]}, ones, x, false);
-  return x;
+  for (int j = 0; j < 8; ++j) rest[j] = p[8 * k + j] - (float)hi[j];
+  return pack8(rest, 0);
 }
 
-// Scores into weights p, which carry 2^-m of their own, and their sum; what m moved by is
+// acc += values of 16 keys times a term of their weights
+template <int D>
+DEV_INLINE void add_values(f32x16 (&acc)[D / 32], const bf16v8 (&v)[D / 32], const bf16v8& p) {
+  #pragma unroll
+  for (int dt = 0; dt < D / 32; ++dt) acc[dt] = mfma(v[dt], p, acc[dt]);
+}
+
+// Scores into weights, first terms into hi. They carry 2^-m of their own, and their sum; what m moved by is
 // returned, and what was weighed before is to be rescaled by 2 to that.
 // m is a whole number and may lag by 8: weights that differ by powers of two round alike,
 // so that tiles and slices do not change the result beyond the order of fp32 sums, and
-// sums are hardly ever rescaled. The sum is of the weights before they are rounded, whose
-// errors are even; of rows that see 16 keys at most (few) it is of the rounded ones, whose
-// errors cancel then (a single key's value comes out as it is).
+// sums are hardly ever rescaled. Nothing is lost by a leading weight that is not 1, as its
+// two terms carry 17 bits of it.
 template <int NS>
-DEV_INLINE float weigh(f32x16 (&st)[NS], bf16v8 (&p)[NS][2], float& m, float& sum, bool few,
-                       float scale_log2) {
+DEV_INLINE float weigh(f32x16 (&st)[NS], bf16v8 (&hi)[NS][2], float& m, float& sum, float scale_log2) {
   float mx = st[0][0];
   #pragma unroll
   for (int n = 0; n < NS; ++n)
@@ -199,15 +206,7 @@ DEV_INLINE float weigh(f32x16 (&st)[NS], bf16v8 (&p)[NS][2], float& m, float& su
       sum += st[n][j];
     }
     #pragma unroll
-    for (int k2 = 0; k2 < 2; ++k2) p[n][k2] = pack8(st[n], k2);
-  }
-  if (__any(few)) {
-    float rounded = 0.f;
-    #pragma unroll
-    for (int n = 0; n < NS; ++n)
-      #pragma unroll
-      for (int k2 = 0; k2 < 2; ++k2) rounded = pair_sum(p[n][k2], rounded);
-    sum = few ? rounded : sum;
+    for (int k2 = 0; k2 < 2; ++k2) hi[n][k2] = pack8(st[n], k2);
   }
   return fall;
 }
@@ -340,18 +339,21 @@ void chunk_attn_kernel(Chunk a) {
           #pragma unroll
           for (int n = 0; n < NS; ++n) hide(st[n], w, k0 + n * 32);
         }
-        bf16v8 p[NS][2];
+        bf16v8 hi[NS][2];
         float sum;
-        const float fall = weigh(st, p, m, sum, w.mine <= FEW, a.scale_log2);
+        const float fall = weigh(st, hi, m, sum, a.scale_log2);
         if (__any(fall < 0.f)) rescale<D>(fall, lsum, acc);
         lsum += sum;
         #pragma unroll
         for (int n = 0; n < NS; ++n)
           #pragma unroll
-          for (int k2 = 0; k2 < 2; ++k2)
+          for (int k2 = 0; k2 < 2; ++k2) {
+            bf16v8 v[D / 32];
             #pragma unroll
-            for (int dt = 0; dt < D / 32; ++dt)
-              acc[dt] = mfma(fr.col(vt, n * 32 + k2 * 16, dt), p[n][k2], acc[dt]);
+            for (int dt = 0; dt < D / 32; ++dt) v[dt] = fr.col(vt, n * 32 + k2 * 16, dt);
+            add_values<D>(acc, v, hi[n][k2]);
+            add_values<D>(acc, v, rest8(st[n], hi[n][k2], k2));
+          }
       }
       if (more) {
         char* next = smem + (turn ^ 1) * (2 * TB);
@@ -401,16 +403,19 @@ void chunk_few_kernel(Chunk a) {
         #pragma unroll
         for (int ks = 0; ks < D / 16; ++ks) st[0] = mfma(fr.row(smem, wave, ks), qf[ks], st[0]);
         if (k0 + 32 > min(w.least, w.end)) hide(st[0], w, k0);
-        bf16v8 p[1][2];
+        bf16v8 hi[1][2];
         float sum;
-        const float fall = weigh(st, p, m, sum, w.mine <= FEW, a.scale_log2);
+        const float fall = weigh(st, hi, m, sum, a.scale_log2);
         if (__any(fall < 0.f)) rescale<D>(fall, lsum, acc);
         lsum += sum;
         #pragma unroll
-        for (int k2 = 0; k2 < 2; ++k2)
+        for (int k2 = 0; k2 < 2; ++k2) {
+          bf16v8 v[D / 32];
           #pragma unroll
-          for (int dt = 0; dt < D / 32; ++dt)
-            acc[dt] = mfma(fr.col(smem + TB, wave * 32 + k2 * 16, dt), p[0][k2], acc[dt]);
+          for (int dt = 0; dt < D / 32; ++dt) v[dt] = fr.col(smem + TB, wave * 32 + k2 * 16, dt);
+          add_values<D>(acc, v, hi[0][k2]);
+          add_values<D>(acc, v, rest8(st[0], hi[0][k2], k2));
+        }
       }
       __syncthreads();
     }
@@ -671,12 +676,12 @@ void chunk_deep_kernel(Chunk a) {
       read_values(0);
       if (careful) hide(st[0], w, k0);
       scores(next);             // past the end of what lies there, unused
-      bf16v8 p[1][2];
+      bf16v8 hi[1][2];
       float sum;
-      const float fall = weigh(st, p, m, sum, w.mine <= FEW, a.scale_log2);
+      const float fall = weigh(st, hi, m, sum, a.scale_log2);
       // here, and not behind the branch
-      hold(p[0][0]);
-      hold(p[0][1]);
+      hold(hi[0][0]);
+      hold(hi[0][1]);
       #pragma unroll
       for (int dt = 0; dt < D / 32; ++dt) hold(v[0][dt]);
       if (__any(fall < 0.f)) rescale<D>(fall, lsum, acc);
@@ -684,9 +689,9 @@ void chunk_deep_kernel(Chunk a) {
       read_values(1);
       read_keys(i + 2);
       #pragma unroll
-      for (int k2 = 0; k2 < 2; ++k2)
-        #pragma unroll
-        for (int dt = 0; dt < D / 32; ++dt) acc[dt] = mfma(v[k2][dt], p[0][k2], acc[dt]);
+      for (int k2 = 0; k2 < 2; ++k2) add_values<D>(acc, v[k2], hi[0][k2]);
+      #pragma unroll
+      for (int k2 = 0; k2 < 2; ++k2) add_values<D>(acc, v[k2], rest8(st[0], hi[0][k2], k2));
       landed<4 * PER>();
       if (careful) {
         tile.mend(tile.keys(i + 3), tile.lines_of(i + 3));
