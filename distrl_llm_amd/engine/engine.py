@@ -202,7 +202,13 @@ class Engine:
         device, total, bs = self.device, sum(new), self.pool.block_size
         if total == 0:
             raise ValueError("a prompt phase without a token")
+        # prompts of which the cache holds nothing first: their rows are those
+        # before `split`
+        order = sorted(range(len(seqs)), key=lambda i: seqs[i].context_len > 0)
+        seqs, new = [seqs[i] for i in order], [new[i] for i in order]
         cached = [q.context_len for q in seqs]
+        fresh = cached.count(0)
+        split = sum(new[:fresh])
         for q, n in zip(seqs, new):
             q.context_len += n
             while len(q.block_table) < KVCachePool.blocks_for(q.context_len, bs):
@@ -223,22 +229,37 @@ class Engine:
         plan = OF.chunk_slots(tables, ctx, lens, pages, bs, total, held)
         input_ids, positions, slot_mapping = ids.long(), plan.positions, plan.slots
 
+        tails = ((tables[fresh:], plan.cu[fresh:] - split, plan.context_lens[fresh:])
+                 if split < total else None)
+
+        def own_rows(q, k, v):
+            if packs:
+                return ext.flash_attn_varlen(q, k, v, plan.cu[:fresh + 1],
+                                             max(new[:fresh]), self.scale)
+            return self._prefill_attention(q, k, v, new[:fresh])
+
         def attend(q, k, v, li):
             """Attention of the step's rows: over the pages where the cache held
-            tokens before them, else over the rows themselves."""
-            if any(cached):
-                return OF.paged_attention_chunk(
-                    q, self.pool.key[li], self.pool.value[li], tables, plan.cu,
-                    plan.context_lens, self.scale, max(new))
-            if packs:
-                return ext.flash_attn_varlen(q, k, v, plan.cu, max(new), self.scale)
-            return self._prefill_attention(q, k, v, new)
+            tokens before them, else over the rows themselves, as if no other
+            prompt of the step had anything cached."""
+            if tails is None:
+                return own_rows(q, k, v)
+            over = OF.paged_attention_chunk(
+                q[split:], self.pool.key[li], self.pool.value[li], *tails, self.scale,
+                max(new[fresh:]))
+            if split == 0:
+                return over
+            return torch.cat([own_rows(q[:split], k[:split], v[:split]), over])
 
+        last = plan.last
+        if order != sorted(order):              # rows back in the caller's order
+            last = last[torch.tensor(sorted(range(len(order)), key=order.__getitem__),
+                                     device=device)]
         packs = self._prefill_packs()
         if packs:
             ext = OF._require_ext("prefill")
             x = self._prefill_packed(input_ids, positions, slot_mapping, attend)
-            return self.model.logits(x[plan.last])
+            return self.model.logits(x[last])
         x = self.model.model.embed_tokens(input_ids)
         for li, layer in enumerate(self.model.model.layers):
             h = layer.input_layernorm(x)
@@ -258,7 +279,7 @@ class Engine:
             u = self._proj(layer.mlp.up_proj, h2)
             x = x + self._proj(layer.mlp.down_proj, OF.silu_mul(g, u))
         x = self.model.model.norm(x)
-        return self.model.logits(x[plan.last])
+        return self.model.logits(x[last])
 
     def _prefill_packs(self) -> bool:
         """Whether the prompt phase can run on packed rows: bf16 on the GPU,

@@ -1,0 +1,66 @@
+"""What a prompt phase of the dense engine runs through, prompt by prompt: none is
+computed another way because of what is cached of the others."""
+
+import pytest
+import torch
+
+from distrl_llm_amd.ops import functional as OF
+from test_chunked_prefill import _engine, _model, _prefill, _prompts
+
+HEAD = list(range(300, 333))        # four whole pages of 8
+
+
+@pytest.fixture(scope="module")
+def tiny():
+    return _model("tiny-qwen2", torch.device("cpu"), torch.float32)
+
+
+def _with_head_cached(model, **kw):
+    engine = _engine(model, 0, cache=True, **kw)
+    _prefill(engine, [HEAD])
+    return engine
+
+
+MIXES = [(0, 1), (1, 0), (1, 0, 0, 1, 1), (0, 0, 1, 0)]       # 1: behind the cached head
+
+
+def _mix(kinds):
+    return [HEAD * kind + p
+            for kind, p in zip(kinds, _prompts((9, 14, 3, 21, 6), 2048, len(kinds)))]
+
+
+@pytest.mark.parametrize("kinds", MIXES)
+def test_fresh_prompts_keep_their_attention(tiny, monkeypatch, kinds):
+    """Beside cached ones they attend over their own rows, and logits come in the
+    order of the prompts."""
+    prompts = _mix(kinds)
+    want, _ = _prefill(_engine(tiny, 0), prompts)
+    engine = _with_head_cached(tiny)
+    own, chunks = [], []
+    attention, chunk = engine._prefill_attention, OF.paged_attention_chunk
+    monkeypatch.setattr(engine, "_prefill_attention",
+                        lambda q, k, v, lens: own.append(lens) or attention(q, k, v, lens))
+    monkeypatch.setattr(OF, "paged_attention_chunk",
+                        lambda q, *args: chunks.append(len(q)) or chunk(q, *args))
+    got, _ = _prefill(engine, prompts)
+    # two orders of the same fp32 sums of some hundred terms
+    assert float((got - want).abs().max()) <= 2.0 ** -14 * float(want.abs().max())
+    layers = tiny.spec.num_layers
+    assert own == [[len(p) for p, kind in zip(prompts, kinds) if not kind]] * layers
+    assert chunks == [sum(len(p) - 32 for p, kind in zip(prompts, kinds) if kind)] * layers
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("packs", [True, False])
+@pytest.mark.parametrize("kinds", MIXES)
+def test_fresh_prompts_beside_cached_ones_gpu(kinds, packs):
+    """As between the packed and the module path: 2 % of the norm, row by row."""
+    model = _model("small-qwen2", torch.device("cuda"), torch.bfloat16, 8)
+    prompts = _mix(kinds)
+    want, _ = _prefill(_engine(model, 0, device="cuda"), prompts)
+    engine = _with_head_cached(model, device="cuda")
+    if not packs:
+        engine._prefill_packs = lambda: False
+    got, _ = _prefill(engine, prompts)
+    for x, y in zip(got.float(), want.float()):
+        assert float((x - y).norm() / y.norm()) < 0.02
