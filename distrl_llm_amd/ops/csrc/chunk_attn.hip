@@ -221,6 +221,11 @@ DEV_INLINE void rescale(float fall, float& lsum, f32x16 (&acc)[D / 32]) {
     for (int j = 0; j < 16; ++j) acc[dt][j] *= alpha;
 }
 
+// The sum of a part in which a row sees no key; told by its bits, as a sum that is no number
+// (a query's that is none) is neither more nor less than any.
+constexpr float NONE = -1.f;
+DEV_INLINE bool is_none(float sum) { return __float_as_uint(sum) == __float_as_uint(NONE); }
+
 // This lane's row, or its part of it, into memory.
 template <int D>
 DEV_INLINE void finish(const Chunk& a, const Work& w, float m, float lsum, f32x16 (&acc)[D / 32]) {
@@ -241,8 +246,8 @@ DEV_INLINE void finish(const Chunk& a, const Work& w, float m, float lsum, f32x1
   const int64_t part = blockIdx.y * (int64_t)a.T * a.H + at;
   if (w.begin < w.end) store_rows_f32<D>(acc, a.o_part + part * D, w.live);
   if ((threadIdx.x & 63) < 32 && w.live) {
-    a.ml_part[part * 2] = seen ? m : -1e30f;
-    a.ml_part[part * 2 + 1] = lsum;
+    a.ml_part[part * 2] = m;
+    a.ml_part[part * 2 + 1] = seen ? lsum : NONE;
   }
 }
 
@@ -429,19 +434,22 @@ void chunk_few_kernel(Chunk a) {
   if (l < 32) {
     const bool seen = min(w.mine, w.end) > w.begin + wave * 32;
     ml[(wave * WROWS + l) * 2] = seen ? m : -1e30f;
-    ml[(wave * WROWS + l) * 2 + 1] = seen ? lsum : 0.f;
+    ml[(wave * WROWS + l) * 2 + 1] = seen ? lsum : NONE;
   }
   __syncthreads();
   const int row = threadIdx.x / 8, r = w.block0 + row, of = a.by_group.of(r);
   if (r >= w.rows) return;
   float top = -1e30f, total = 0.f, f[NW];
+  bool seen[NW], any = false;
   #pragma unroll
   for (int i = 0; i < NW; ++i) top = fmaxf(top, ml[(i * WROWS + row) * 2]);
   #pragma unroll
   for (int i = 0; i < NW; ++i) {
     const float sum = ml[(i * WROWS + row) * 2 + 1];
-    f[i] = sum > 0.f ? __builtin_amdgcn_exp2f(ml[(i * WROWS + row) * 2] - top) : 0.f;
-    total += f[i] * sum;
+    seen[i] = !is_none(sum);
+    any |= seen[i];
+    f[i] = __builtin_amdgcn_exp2f(ml[(i * WROWS + row) * 2] - top);
+    total += seen[i] ? f[i] * sum : 0.f;
   }
   const int64_t at = (int64_t)(w.q.first + of) * a.H + kv * a.by_group.n + r - of * a.by_group.n;
   const int64_t part = blockIdx.y * (int64_t)a.T * a.H + at;
@@ -451,13 +459,13 @@ void chunk_few_kernel(Chunk a) {
     f32x4 o = {0.f, 0.f, 0.f, 0.f};
     #pragma unroll
     for (int i = 0; i < NW; ++i)
-      if (f[i] > 0.f)           // else what is there is no number
+      if (seen[i])              // else what is there is no number
         o += f[i] * *reinterpret_cast<const f32x4*>(parts + (i * WROWS + row) * LD + d);
     if (gridDim.y > 1) {
       *reinterpret_cast<f32x4*>(a.o_part + part * D + d) = o;
       continue;
     }
-    const float inv = total > 0.f ? 1.f / total : 0.f;
+    const float inv = any ? 1.f / total : 0.f;
     bf16v4 y;
     #pragma unroll
     for (int j = 0; j < 4; ++j) y[j] = (__bf16)(o[j] * inv);
@@ -465,7 +473,7 @@ void chunk_few_kernel(Chunk a) {
   }
   if (gridDim.y > 1 && threadIdx.x % 8 == 0) {
     a.ml_part[part * 2] = top;
-    a.ml_part[part * 2 + 1] = total;
+    a.ml_part[part * 2 + 1] = any ? total : NONE;
   }
 }
 
@@ -726,9 +734,11 @@ void chunk_join_kernel(Chunk a, int slices) {
   const int t = (int)(row / a.H);
   if (t < a.first(0) || t >= a.first(a.B)) return;
   float m = -1e30f, l = 0.f, o[8] = {};
+  bool any = false;
   for (int z = 0; z < slices; ++z) {
     const float2 ml = reinterpret_cast<const float2*>(a.ml_part)[z * n + row];
-    if (ml.y == 0.f) continue;
+    if (is_none(ml.y)) continue;
+    any = true;
     const float m_new = fmaxf(m, ml.x);
     const float keep = __builtin_amdgcn_exp2f(m - m_new), add = __builtin_amdgcn_exp2f(ml.x - m_new);
     const f32x4* p = reinterpret_cast<const f32x4*>(a.o_part + (z * n + row) * D + i % (D / 8) * 8);
@@ -739,7 +749,7 @@ void chunk_join_kernel(Chunk a, int slices) {
   }
   bf16x8 out;
   #pragma unroll
-  for (int j = 0; j < 8; ++j) out.v[j] = f2bf(l > 0.f ? o[j] / l : 0.f);
+  for (int j = 0; j < 8; ++j) out.v[j] = f2bf(any ? o[j] / l : 0.f);
   *reinterpret_cast<bf16x8*>(a.out + row * D + i % (D / 8) * 8) = out;
 }
 

@@ -171,9 +171,11 @@ def paged_attention_chunk(q, key_cache, value_cache, block_tables, cu,
     context_lens (B,) its tokens in the cache with the new ones. The token at
     position p sees keys 0 .. p, as far as its table reaches; a page number
     outside the cache reads as zeros, a token that sees no key and rows of no
-    sequence give zeros. Cached values a sequence has have to be finite; what
-    lies behind its end or on other pages may be anything. ``longest``: the
-    most rows of one sequence; it picks the kernel, not the result's rows.
+    sequence give zeros. A query that holds no number or an infinite one makes
+    its row and head NaN, no other. Cached values a sequence has have to be
+    finite; what lies behind its end or on other pages may be anything.
+    ``longest``: the most rows of one sequence; it picks the kernel, not the
+    result's rows.
 
     bfloat16 and head_dim 64 or 128 on the GPU. No gradient: the cache serves
     generation."""
