@@ -790,7 +790,10 @@ torch::Tensor paged_attention_chunk(torch::Tensor q, torch::Tensor kcache, torch
   for (const auto* t : {&kcache, &vcache})
     TORCH_CHECK(reinterpret_cast<uintptr_t>(t->data_ptr()) % 16 == 0,
                 "paged_attention_chunk: caches on 16 bytes");
-  TORCH_CHECK(scale > 0. && scale < 1e30, "paged_attention_chunk: a positive scale");
+  // hidden scores are -1e30 before they are scaled, and have to be far below the others then;
+  // scaled ones have to stay within 2^29, as a larger maximum's rounding is no weight's
+  // exponent any more
+  TORCH_CHECK(scale >= 1e-12 && scale <= 1e6, "paged_attention_chunk: a scale of 1e-12 to 1e6");
   TORCH_CHECK(longest >= 0, "paged_attention_chunk: longest");
   TORCH_CHECK(T * H < (1ll << 30) && kcache.size(0) * kcache.size(1) < (1ll << 31) && B < (1 << 24),
               "paged_attention_chunk: too many rows");

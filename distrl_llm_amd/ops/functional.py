@@ -177,14 +177,14 @@ def paged_attention_chunk(q, key_cache, value_cache, block_tables, cu,
     ``longest``: the most rows of one sequence; it picks the kernel, not the
     result's rows.
 
-    bfloat16 and head_dim 64 or 128 on the GPU. No gradient: the cache serves
-    generation."""
+    bfloat16 and head_dim 64 or 128 on the GPU. ``scale``: 1e-12 to 1e6, and
+    scale times q.k within 2^29. No gradient: the cache serves generation."""
     if torch.is_grad_enabled() and (q.requires_grad or key_cache.requires_grad
                                     or value_cache.requires_grad):
         raise RuntimeError("paged_attention_chunk has no gradient: call it "
                            "under torch.no_grad()")
-    if not 0.0 < scale < 1e30 or longest < 0:
-        raise ValueError("paged_attention_chunk: a positive scale, longest >= 0")
+    if not 1e-12 <= scale <= 1e6 or longest < 0:
+        raise ValueError("paged_attention_chunk: a scale of 1e-12 to 1e6, longest >= 0")
     if q.is_cuda:
         ext = _require_ext("paged_attention_chunk")
         if ext is not None:
