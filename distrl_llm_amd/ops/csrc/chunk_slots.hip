@@ -29,15 +29,27 @@ struct Slots {
   int B, width, block, free, rows;
 };
 
-struct Need { int tokens, pages; };
+// Sums stop at MANY: lengths may be any numbers, and there are fewer rows and free pages.
+constexpr uint32_t MANY = 0x7fffffff;
+struct Need {
+  int tokens, pages;
+  DEV_INLINE static int sum(int a, int b) { return (int)min((uint32_t)a + (uint32_t)b, MANY); }
+  DEV_INLINE void operator+=(const Need& n) {
+    tokens = sum(tokens, n.tokens);
+    pages = sum(pages, n.pages);
+  }
+};
 
-DEV_INLINE int pages_of(int n, int block) { return n <= 0 ? 0 : (n - 1) / block + 1; }
+DEV_INLINE int pages_of(uint32_t n, int block) {
+  return n == 0 ? 0 : (int)min((n - 1) / (uint32_t)block + 1, MANY);
+}
 DEV_INLINE int held_of(const Slots& a, int b) {
-  return max(0, a.held ? a.held[b] : pages_of(a.ctx[b], a.block));
+  return max(0, a.held ? a.held[b] : pages_of(max(0, a.ctx[b]), a.block));
 }
 DEV_INLINE Need need_of(const Slots& a, int b) {
   const int n = max(0, a.fresh[b]);
-  return {n, max(0, pages_of(a.ctx[b] + n, a.block) - held_of(a, b))};
+  const int64_t with = (int64_t)a.ctx[b] + n;           // below 2^32
+  return {n, max(0, pages_of((uint32_t)max(with, (int64_t)0), a.block) - held_of(a, b))};
 }
 
 // the largest b < n with sum[b] <= i; sums never fall, sum[0] = 0
@@ -68,15 +80,15 @@ struct Place {
       ctx = a.ctx[b];
       held = held_of(a, b);
     }
-    position = ctx + i - cu[b];
+    position = (int)((uint32_t)ctx + (uint32_t)(i - cu[b]));
     if (position < 0) return -1;
     const int p = position / a.block;
     if (p != page_index) {
       page_index = p;
-      const int from = opened[b] + p - held;
+      const uint32_t from = (uint32_t)opened[b] + (uint32_t)(p - held);
       page = p >= a.width ? -1
              : p < held   ? a.tables[(int64_t)b * a.width + p]
-             : (unsigned)from < (unsigned)a.free ? a.pages[from] : -1;
+             : from < (uint32_t)a.free ? a.pages[from] : -1;
     }
     return page >= 0 ? (int64_t)page * a.block + (position - p * a.block) : -1;
   }
@@ -98,32 +110,23 @@ void chunk_slots_kernel(Slots a) {
   // a run of requests a thread, then the runs' sums over the workgroup
   const int run = CDIV(a.B, THREADS), b0 = min(tid * run, a.B), b1 = min(b0 + run, a.B);
   Need sum{0, 0};
-  for (int b = b0; b < b1; ++b) {
-    sum.tokens += cu[b];
-    sum.pages += opened[b];
-  }
+  for (int b = b0; b < b1; ++b) sum += Need{cu[b], opened[b]};
   Need to = sum;                // inclusive over the wave
   #pragma unroll
   for (int off = 1; off < WAVE; off <<= 1) {
-    const int t = __shfl_up(to.tokens, off, WAVE), p = __shfl_up(to.pages, off, WAVE);
-    if (lane >= off) {
-      to.tokens += t;
-      to.pages += p;
-    }
+    const Need before{__shfl_up(to.tokens, off, WAVE), __shfl_up(to.pages, off, WAVE)};
+    if (lane >= off) to += before;
   }
   if (lane == WAVE - 1) wave_sum_of[wave] = to;
   __syncthreads();
-  Need at{to.tokens - sum.tokens, to.pages - sum.pages};
-  for (int w = 0; w < wave; ++w) {
-    at.tokens += wave_sum_of[w].tokens;
-    at.pages += wave_sum_of[w].pages;
-  }
+  Need at{__shfl_up(to.tokens, 1, WAVE), __shfl_up(to.pages, 1, WAVE)};
+  if (lane == 0) at = Need{0, 0};
+  for (int w = 0; w < wave; ++w) at += wave_sum_of[w];
   for (int b = b0; b < b1; ++b) {
     const Need n{cu[b], opened[b]};
     cu[b] = at.tokens;
     opened[b] = at.pages;
-    at.tokens += n.tokens;
-    at.pages += n.pages;
+    at += n;
   }
   if (tid == THREADS - 1) {
     cu[a.B] = at.tokens;
@@ -160,14 +163,25 @@ void chunk_slots_kernel(Slots a) {
       }
     }
   }
-  for (int i = me; i < opened[a.B]; i += stride) {
-    const int b = find(opened, a.B, i), p = held_of(a, b) + i - opened[b];
-    if ((unsigned)p < (unsigned)a.width) a.tables[(int64_t)b * a.width + p] = i < a.free ? a.pages[i] : -1;
+  const int64_t entries = (int64_t)a.B * a.width;
+  if (opened[a.B] <= entries) {
+    for (int64_t i = me; i < opened[a.B]; i += stride) {
+      const int b = find(opened, a.B, (int)i);
+      const int64_t p = held_of(a, b) + i - opened[b];
+      if (p < a.width) a.tables[(int64_t)b * a.width + p] = i < a.free ? a.pages[i] : -1;
+    }
+  } else {                      // more than the tables can take: by their entries
+    for (int64_t e = me; e < entries; e += stride) {
+      const int b = (int)(e / a.width), of = (int)(e - (int64_t)b * a.width) - held_of(a, b);
+      if ((uint32_t)of >= (uint32_t)need_of(a, b).pages) continue;
+      const uint32_t from = (uint32_t)opened[b] + (uint32_t)of;
+      a.tables[e] = from < (uint32_t)a.free ? a.pages[from] : -1;
+    }
   }
   for (int b = me; b <= a.B; b += stride) {
     a.cu[b] = min(cu[b], a.rows);
     if (b == a.B) break;
-    a.context[b] = a.ctx[b] + max(0, a.fresh[b]);
+    a.context[b] = (int)((uint32_t)a.ctx[b] + (uint32_t)max(0, a.fresh[b]));
     a.last[b] = min(max(cu[b + 1], 1), max(a.rows, 1)) - 1;
   }
 }

@@ -155,15 +155,14 @@ def chunk_slots(block_tables: torch.Tensor, context_lens: torch.Tensor,
     positions, slots, cu = [], [], [0]
     for b, (ctx, new) in enumerate(zip(context_lens.tolist(), new_lens.tolist())):
         new = max(new, 0)
-        have = -(-ctx // block_size) if held is None else int(held[b])
+        have = max(-(-ctx // block_size) if held is None else int(held[b]), 0)
+        need = max(-(-(ctx + new) // block_size) - have, 0)
         table = block_tables[b].tolist()
-        for p in range(max(have, 0), -(-(ctx + new) // block_size)):
-            page = free[at] if at < len(free) else -1
-            at += 1
-            if p < width:
-                table[p] = page
+        for i in range(min(need, max(width - have, 0))):
+            table[have + i] = free[at + i] if at + i < len(free) else -1
+        at += need
         block_tables[b] = torch.tensor(table, dtype=torch.int32, device=dev)
-        for position in range(ctx, ctx + new):
+        for position in range(ctx, ctx + min(new, max(rows - len(slots), 0))):
             p = position // block_size
             page = table[p] if 0 <= p < width else -1
             positions.append(position)
