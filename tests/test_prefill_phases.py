@@ -64,3 +64,51 @@ def test_fresh_prompts_beside_cached_ones_gpu(kinds, packs):
     got, _ = _prefill(engine, prompts)
     for x, y in zip(got.float(), want.float()):
         assert float((x - y).norm() / y.norm()) < 0.02
+
+
+TAILS = [(1,), (2,), (1, 2, 1), (1,) * 20, (4,), (1, 2) * 6]
+
+
+def _tails(lengths):
+    return [HEAD[:32] + p for p in _prompts(lengths, 2048, 9)]
+
+
+@pytest.mark.parametrize("lengths", TAILS)
+def test_few_tokens_go_through_decode_steps(tiny, monkeypatch, lengths):
+    """A token of each prompt a step, where that is the faster; more in one pass."""
+    want, rows = _prefill(_engine(tiny, 0), _tails(lengths))
+    engine, steps, passes = _with_head_cached(tiny), [], []
+    step, chunk = engine._decode_forward, OF.paged_attention_chunk
+    monkeypatch.setattr(engine, "_decode_forward",
+                        lambda ids, *args: steps.append(len(ids)) or step(ids, *args))
+    monkeypatch.setattr(OF, "paged_attention_chunk",
+                        lambda q, *args: passes.append(len(q)) or chunk(q, *args))
+    got, got_rows = _prefill(engine, _tails(lengths))
+    by_steps = max(lengths) == 1 or max(lengths) == 2 and len(lengths) <= 8
+    assert steps == ([sum(n > i for n in lengths) for i in range(max(lengths))]
+                     if by_steps else [])
+    assert passes == ([] if by_steps else [sum(lengths)] * tiny.spec.num_layers)
+    for x, y in ((got, want), (got_rows, rows)):
+        assert float((x - y).abs().max()) <= 2.0 ** -14 * float(y.abs().max())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("lengths", TAILS)
+def test_few_tokens_gpu(lengths):
+    """As between decode and the prompt phase: 2 % of the norm, row by row."""
+    model = _model("small-qwen2", torch.device("cuda"), torch.bfloat16, 8)
+    want, _ = _prefill(_engine(model, 0, device="cuda"), _tails(lengths))
+    got, _ = _prefill(_with_head_cached(model, device="cuda"), _tails(lengths))
+    for x, y in zip(got.float(), want.float()):
+        assert float((x - y).norm() / y.norm()) < 0.02
+
+
+def test_sequences_end_where_they_are(tiny):
+    """Tables, contexts and a generated token behind a tail of one."""
+    from distrl_llm_amd.config import SamplingParams
+    sp = SamplingParams(max_tokens=4, temperature=0.0, n=2)
+    prompts = _tails((1, 1)) + [HEAD[:24] + [5]]
+    want = _engine(tiny, 0).generate(prompts, sp, eos_token_id=None)
+    engine = _with_head_cached(tiny)
+    assert engine.generate(prompts, sp, eos_token_id=None) == want
+    engine.clear_prefix_cache()
