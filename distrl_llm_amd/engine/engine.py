@@ -189,15 +189,22 @@ class Engine:
                     break
             lg = self._prefill_step([seqs[i] for i, _ in take],
                                     [n for _, n in take])
-            for row, (i, _) in enumerate(take):
-                if seqs[i].context_len == len(seqs[i].prompt_ids):
-                    logits[i] = lg[row:row + 1]
-                    waiting.remove(i)
+            ended = [i for i, _ in take if self._ended(seqs[i])]
+            for row, i in enumerate(ended):
+                logits[i] = lg[row:row + 1]
+                waiting.remove(i)
         return torch.cat(logits, 0)
 
-    def _prefill_step(self, seqs: List[Sequence], new: List[int]) -> torch.Tensor:
+    @staticmethod
+    def _ended(seq: Sequence) -> bool:
+        """Whether the whole prompt is in the cache."""
+        return seq.context_len == len(seq.prompt_ids)
+
+    def _prefill_step(self, seqs: List[Sequence],
+                      new: List[int]) -> Optional[torch.Tensor]:
         """The next new[i] prompt tokens of every sequence through the layers,
-        their keys and values into the pool -> each one's last row's logits."""
+        their keys and values into the pool -> last-token logits of the prompts
+        that end with them, or None where none does."""
         s = self.spec
         device, total, bs = self.device, sum(new), self.pool.block_size
         if total == 0:
@@ -254,14 +261,16 @@ class Engine:
             return torch.cat([own_rows(q[:split], k[:split], v[:split]), over])
 
         last = plan.last
-        if order != sorted(order):              # rows back in the caller's order
-            last = last[torch.tensor(sorted(range(len(order)), key=order.__getitem__),
-                                     device=device)]
+        # the caller's order, without prompts that go on
+        rows = [i for i in sorted(range(len(order)), key=order.__getitem__)
+                if self._ended(seqs[i])]
+        if rows and rows != list(range(len(order))):
+            last = last[torch.tensor(rows, device=device)]
         packs = self._prefill_packs()
         if packs:
             ext = OF._require_ext("prefill")
             x = self._prefill_packed(input_ids, positions, slot_mapping, attend)
-            return self.model.logits(x[last])
+            return self.model.logits(x[last]) if rows else None
         x = self.model.model.embed_tokens(input_ids)
         for li, layer in enumerate(self.model.model.layers):
             h = layer.input_layernorm(x)
@@ -281,7 +290,7 @@ class Engine:
             u = self._proj(layer.mlp.up_proj, h2)
             x = x + self._proj(layer.mlp.down_proj, OF.silu_mul(g, u))
         x = self.model.model.norm(x)
-        return self.model.logits(x[last])
+        return self.model.logits(x[last]) if rows else None
 
     def _few_tokens(self, seqs: List[Sequence], new: List[int]) -> bool:
         """Whether so few tokens of cached prompts go through decode steps, a
@@ -309,7 +318,8 @@ class Engine:
                                      [seqs[j].context_len for j in live])
             for row, j in enumerate(live):
                 logits[j] = lg[row:row + 1]
-        return torch.cat(logits, 0)
+        ended = [lg for q, lg in zip(seqs, logits) if self._ended(q)]
+        return torch.cat(ended, 0) if ended else None
 
     def _prefill_packs(self) -> bool:
         """Whether the prompt phase can run on packed rows: bf16 on the GPU,

@@ -112,3 +112,16 @@ def test_sequences_end_where_they_are(tiny):
     engine = _with_head_cached(tiny)
     assert engine.generate(prompts, sp, eos_token_id=None) == want
     engine.clear_prefix_cache()
+
+
+def test_only_prompts_that_end_have_logits(tiny, monkeypatch):
+    """A chunk that does not end its prompt asks for no row of the vocabulary."""
+    prompts = _prompts((20, 3, 30, 1), 2048)
+    want, _ = _prefill(_engine(tiny, 0), prompts)
+    engine, rows = _engine(tiny, 8), []
+    logits = tiny.logits
+    monkeypatch.setattr(tiny, "logits", lambda x: rows.append(len(x)) or logits(x))
+    # steps of [8], [8], [4, 3, 1], [8], [8], [8], [5, 1]
+    got, _ = _prefill(engine, prompts)
+    assert rows == [2, 2]
+    assert float((got - want).abs().max()) <= 2.0 ** -14 * float(want.abs().max())
