@@ -1032,6 +1032,16 @@ class Engine:
                     else:
                         running.append(c)
 
+        def admit_first():
+            """Admissions until a sequence runs or no prompt waits; those of an
+            admission may all have ended with their first token."""
+            while waiting and not running:
+                before = len(waiting)
+                try_admit()
+                if not running and len(waiting) == before:
+                    raise MemoryError(
+                        "KV pool too small to admit any waiting prompt")
+
         try_admit()
 
         force_session = os.environ.get("DISTRL_FORCE_SESSION") == "1"
@@ -1050,11 +1060,8 @@ class Engine:
             retire_unit = int(os.environ.get("DISTRL_RETIRE_UNIT", "16"))
             while running or waiting:
                 if not running:
-                    try_admit()
+                    admit_first()
                     if not running:
-                        if waiting:
-                            raise MemoryError(
-                                "KV pool too small to admit any waiting prompt")
                         break
                 session = self._make_session(running, sp, eos_token_id)
                 retire_at = retire_unit if retire_unit > 0 else None
@@ -1091,11 +1098,8 @@ class Engine:
 
         while running or waiting:
             if not running:
-                try_admit()
+                admit_first()
                 if not running:
-                    if waiting:
-                        raise MemoryError(
-                            "KV pool too small to admit any waiting prompt")
                     break
             logits = self._decode_step(running)
             next_tokens = OF.sample_tokens(logits, sp.temperature, sp.top_p,
