@@ -172,8 +172,9 @@ class Engine:
         one flat batch, or in steps of up to ``prefill_chunk_tokens`` tokens
         that cut long prompts -> last-token logits (len(seqs), V).
         Behind 1040 cached tokens, ms, token by token through decode steps and
-        so: a tail of 5 tokens 0.5B 4.0, 2.1, 7B 15.6, 5.5; 16 tails of 20 and
-        121 tokens 0.5B 123, 3.5, 7B 432, 20."""
+        so: a tail of 5 tokens 0.5B 4.0, 2.2, 7B 15.6, 5.6; 16 tails of 20 and
+        121 tokens 0.5B 123, 3.5, 7B 433, 20 (generate admits seven of these
+        prompts at a time, as their cached tokens count as well)."""
         budget = self.cfg.prefill_chunk_tokens
         logits: List[Optional[torch.Tensor]] = [None] * len(seqs)
         waiting = list(range(len(seqs)))

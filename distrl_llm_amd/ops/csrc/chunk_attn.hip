@@ -14,14 +14,18 @@
 //
 // Weights go into the second product as two bf16 terms, 17 bits, as those of single tokens
 // do (paged_attn.hip); the result's error against 64 bits is then that of its own rounding
-// (0.00166, with one term 0.0023). It costs half as much matrix work again: 2 x 4096 behind
-// 8192, 64/8 heads of 128 3480 us for 2670, 1180 TFLOP/s with the second terms (a product
-// of 8192^3 1296). Tried there, with one term: 128 rows a workgroup 2796, the light kernel
-// 2975, 64 rows a wave (one wave a SIMD) 3755, twelve waves of 32 (three a SIMD) 2856 for
-// 2767, priorities of waves even. 6 single tokens behind 20 to 32 thousand, 40/8 heads 128
-// us = 4.5 TB/s, K and V read once. 16 x 20..120 behind 1040, 28/4 50 us, 10 x 200..350
-// behind none 24: a workgroup's start (lengths, pages, rows, one behind the other) and 6 to
-// 35 blocks or tiles. 5 tokens behind 1040, 14/2 of 64 11: two launches of such chains.
+// (0.00166, with one term 0.0023). It costs half as much matrix work again. us, one card,
+// one term and two: 2 x 4096 behind 8192, 64/8 heads of 128 2729 and 3584 (1150 TFLOP/s with
+// the second terms, a product of 8192^3 1296); 2048 behind 14336, 28/4 501 and 647; 30 single
+// tokens and 2 x 512 behind up to 2900, 32/8 102 and 119; 16 x 20..121 behind 1040, 28/4 43
+// and 51. The first of these keeps matrix cores and vector units busy for 58 % of the time
+// each; little of one wave's products hides behind the vector work of the SIMD's other.
+// Tried there, with one term (2690): 128 rows a workgroup 2796, the light kernel 2975, 64 rows
+// a wave (one wave a SIMD) 3755, twelve waves of 32 (three a SIMD) 2856 for 2767, priorities
+// of waves even. 6 single tokens behind 20 to 32 thousand, 40/8 heads 129 us = 4.5 TB/s, K and
+// V read once. 16 x 20..121 behind 1040 and 10 x 200..350 behind none, 28/4 (24 us): a
+// workgroup's start (lengths, pages, rows, one behind the other) and up to 36 blocks or 6
+// tiles. 5 tokens behind 1040, 14/2 of 64 10.8: two launches of such chains.
 #include <torch/extension.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -166,7 +170,7 @@ DEV_INLINE void hide(f32x16& st, const Work& w, int k0) {
 
 // The second term of weights 8 k .. 8 k + 7, whose first is hi = pack8(p, k): p = hi + lo,
 // off by 2^-16 of p at most. (Made and used beside the products with hi: with those of both
-// terms behind it all 2 x 4096 behind 8192 take 3816 us for 3480.)
+// terms behind it all 2 x 4096 behind 8192 take 3689 us for 3583.)
 DEV_INLINE bf16v8 rest8(const f32x16& p, const bf16v8& hi, int k) {
   f32x16 rest;
   #pragma unroll
@@ -297,8 +301,9 @@ struct Staged {
 
 // Shorter contexts and fewer rows: tiles of 64 keys, the next one on its way into registers
 // while this one's scores, weights and values follow one another. It starts in half the
-// time of the kernel below. (Two waves a workgroup and tiles of 32: 10 x 200..350 behind
-// none, 28/4 heads 22.7 us for 22.1, 80 x 100 33.8 for 37.4, 4 x 1200 85 for 67.)
+// time of the kernel below. (Two waves a workgroup and tiles of 32, with weights of one term:
+// 10 x 200..350 behind none, 28/4 heads 22.7 us for 22.1, 80 x 100 33.8 for 37.4, 4 x 1200 85
+// for 67.)
 template <int D, int NW>
 __global__ __launch_bounds__(NW * 64, 2)
 void chunk_attn_kernel(Chunk a) {
@@ -848,9 +853,9 @@ torch::Tensor paged_attention_chunk(torch::Tensor q, torch::Tensor kcache, torch
     const int64_t grid = check(grid_of(FEWS ? WROWS : 4 * WROWS));
     // Slices where the workgroups leave CUs idle (a CU holds two of four waves, with heads
     // of 64 four), of 256 keys at least and from three of them on: the join is a launch of 4
-    // us. 5 tokens behind 1040, 14/2 heads of 64 12.2 us, one slice 18. Half and twice as
-    // many: 36 x 43..68 behind up to 8435, 8/2 of 64 92.5 and 57.4, 2 x 36..826 behind 6000,
-    // 32/8 of 128 40.0 and 44.6.
+    // us. 5 tokens behind 1040, 14/2 heads of 64 11.2 us, one slice 12.8. Half, so and twice
+    // as many: 36 x 43..68 behind up to 8435, 8/2 of 64 109, 68 and 63, 2 x 36..826 behind
+    // 6000, 32/8 of 128 45.4, 43.5 and 45.6, 6 x 1 behind 20 to 32 thousand, 40/8 209, 129 and 133.
     const int slices = most < 3 * LEAST ? 1 : (int)std::max<int64_t>(
         1, std::min<int64_t>({(DIM == 64 ? 1024 : 512) / grid, (most + LEAST - 1) / LEAST, 64}));
     torch::Tensor part;
@@ -881,14 +886,18 @@ torch::Tensor paged_attention_chunk(torch::Tensor q, torch::Tensor kcache, torch
   };
   // By rows of a sequence, keys a row sees on average (if sequences are alike and their
   // tables as wide as they need) and workgroups. us, light and deep kernel, 128 rows and
-  // 256 a workgroup: 2 x 4096 behind 8192, 64/8 heads 2975 and 2711; 2048 behind 14336, 28/4
-  // 558 and 503; 8192 behind none, 28/4 538 and 514; 16 x 20..120 behind 1040, 28/4 46.4 and
-  // 44.2; but 4 x 1200 behind none 66.8 and 76.3, 10 x 200..350 22.1 and 30.7, single
-  // tokens among two chunks 99.7 and 138.
+  // 256 a workgroup: 2 x 4096 behind 8192, 64/8 heads 3820 and 3580; 2048 behind 14336, 28/4
+  // 701 and 631; 8192 behind none, 28/4 693 and 661; 16 x 20..121 behind 1040, 28/4 53.2 and
+  // 50.5; but 2 x 1024 behind 2048, 40/8 185 and 199, 4 x 1200 behind none, 28/4 80 and 89,
+  // 512 behind 4096 67 and 167, 10 x 200..350 24.0 and 33.3, single tokens among two chunks
+  // 118 and 162.
   // Up to 64 rows a sequence, where a step waits for chains and not for memory. us, light
-  // kernel and few rows: a token behind 1000, 14/2 heads of 64 10.9 and 9.7, 40/8 of 128
-  // 14.0 and 12.5; 64 x 1 behind 500, 14/2 11.6 and 7.7; but 8 x 1 behind 2000, 28/4 of 128
-  // 18.1 and 20.1, 64 x 1 behind 3000 93.7 and 107 (40/8 207 and 184).
+  // kernel and few rows: a token behind 1000, 14/2 heads of 64 11.5 and 9.9, 40/8 of 128
+  // 14.2 and 12.3; 64 x 1 behind 500, 14/2 12.1 and 7.8, behind 3000 31 and 28; of 128, where a
+  // CU's LDS holds two workgroups, it depends on the batch: 8 x 1 behind 2000, 28/4 18.7
+  // and 19.9, 8 x 5 behind 1040 16.5 and 17.9, 4 x 1 behind 20000, 40/8 72 and 81, 64 x 1
+  // behind 3000, 28/4 103 and 118, but 40/8 223 and 187, 2 x 2 behind 500, 28/4 16.9 and 11.6,
+  // 64 x 5 behind 500, 12/2 17.6 and 12.7.
   const bool few = longest * (H / KV) <= 64 && (D == 64 || B == 1);
   auto by_rows = [&](auto d_) {
     if (few) sliced(d_, std::true_type{});
